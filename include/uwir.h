@@ -256,6 +256,55 @@ int uwir_flash_attn(const void* q, int ldq, const void* k, int ldk, const void* 
                     int ldv2, int dtype, int B, int n, int heads, int hd, float scale, void* o1, int ldo1,
                     void* o2, int ldo2, int out_dtype, void* workspace, size_t workspace_bytes, uwir_stream_t stream);
 
+/* ---- group norm with an activation on NHWC rows, forward and backward (U/attention.py:250-253 nn.GroupNorm as an operator
+ * of its own; the modulated and activated forms and the gradients have no single counterpart in the reference) ----------
+ * x [B*n, ldx >= C] fp32 or bf16, groups G | C, statistics over the n x (C/G) elements of (image, group):
+ *   xh = (x - mean) rstd,  rstd = 1 / sqrt(var + eps)            var biased, as nn.GroupNorm
+ *   z  = (xh gamma + beta) (1 + scale_b) + shift_b               scale_shift [B, ld_ss] = [scale (C) | shift (C)] or NULL
+ *   out = act(z)                                                 UWIR_ACT_NONE or UWIR_ACT_SILU; fp32 or bf16 rows
+ * mean, rstd [B, G] fp32 (each may be NULL) are what the backward pass wants kept.  out may be x itself (same stride and
+ * type).  backward: dy, x, dx share a dtype; dgamma, dbeta [C] fp32 (written, not added to), dscale_shift [B, ld_dss]
+ * [dscale | dshift] or NULL; dx may be dy or x itself.  Statistics and sums are fp32 per thread and fp64 beyond, in a fixed order:
+ * results do not depend on scheduling.  C <= 2048, B <= 65534; any C, strides and element alignment (16-byte aligned
+ * rows with C a multiple of 8 (bf16) or 4 (fp32) run at full width).  workspace (both directions):
+ * >= uwir_group_norm_act_workspace_bytes, 16-byte aligned, contents never carried between calls; calls that may
+ * run at the same time need one each (captured graphs included). */
+size_t uwir_group_norm_act_workspace_bytes(int B, int n, int C, int groups);
+int uwir_group_norm_act(const void* x, int x_dtype, size_t ldx, int B, int n, int C, int groups, float eps, const float* gamma,
+                        const float* beta, const float* scale_shift, size_t ld_ss, int act, void* out, int out_dtype,
+                        size_t ldo, float* mean, float* rstd, void* workspace, size_t workspace_bytes, uwir_stream_t stream);
+int uwir_group_norm_act_backward(const void* dy, size_t ldy, const void* x, size_t ldx, int dtype, int B, int n, int C, int groups,
+                                 const float* gamma, const float* beta, const float* mean, const float* rstd,
+                                 const float* scale_shift, size_t ld_ss, int act, void* dx, size_t ldd, float* dgamma,
+                                 float* dbeta, float* dscale_shift, size_t ld_dss, void* workspace, size_t workspace_bytes,
+                                 uwir_stream_t stream);
+
+/* ---- cross attention to an encoder's states of another length, forward and backward (U/attention.py:152-193
+ * CrossAttention with a context of any length) -----------------------------------------------------------------------
+ * q [B*nq, ldq >= heads*hd], k, v [B*nk, ldk / ldv >= kv_heads*hd]; head h of q reads key / value head
+ * h / (heads / kv_heads) (kv_heads | heads).  A key of image b is visible if its index is below key_lens[b] (int32 [B]
+ * or NULL: nk; values are clamped to [0, nk]) and key_mask[b, index] != 0 (bytes [B, ld_mask >= nk] or NULL: all):
+ *   out = softmax_{visible}(scale q k^T) v [B*nq, ldo],   lse [B, heads, nq] fp32 = log sum_{visible} exp(scale q k) (may be NULL)
+ * An image that shows no key gives out = 0, lse = -inf and zero gradients.  k and v of an invisible key are never used,
+ * whatever they hold; their gradients are written as zeros.  backward: dq, dk, dv (written, not added to) from out, lse of
+ * the forward call and dout; the gradients of shared key heads are summed over their query heads in a fixed order.
+ * All tensors of a call share a dtype (fp32: exact-fp32 MFMA; bf16: bf16 MFMA operands with probabilities and score
+ * gradients rounded to bf16, fp32 accumulation and statistics).  hd % 8 == 0, hd <= 128; rows and strides 16-byte aligned;
+ * scale > 0; nq, nk >= 0; B * kv_heads <= 65535.  Outputs must not overlap any other operand.
+ * workspace: >= the matching *_workspace_bytes (may be 0), 16-byte aligned; calls that may run at the same
+ * time need one each (captured graphs included).  Results do not depend on scheduling. */
+size_t uwir_cross_attn_workspace_bytes(int B, int nq, int nk, int heads, int kv_heads, int hd, int dtype);
+int uwir_cross_attn(const void* q, size_t ldq, const void* k, size_t ldk, const void* v, size_t ldv, int dtype, int B, int nq, int nk,
+                    int heads, int kv_heads, int hd, float scale, const int* key_lens, const unsigned char* key_mask,
+                    size_t ld_mask, void* out, size_t ldo, float* lse, void* workspace, size_t workspace_bytes,
+                    uwir_stream_t stream);
+size_t uwir_cross_attn_backward_workspace_bytes(int B, int nq, int nk, int heads, int kv_heads, int hd, int dtype);
+int uwir_cross_attn_backward(const void* q, size_t ldq, const void* k, size_t ldk, const void* v, size_t ldv, const void* out,
+                             size_t ldo, const float* lse, const void* dout, size_t ld_dout, int dtype, int B, int nq, int nk, int heads,
+                             int kv_heads, int hd, float scale, const int* key_lens, const unsigned char* key_mask,
+                             size_t ld_mask, void* dq, size_t ld_dq, void* dk, size_t ld_dk, void* dv, size_t ld_dv,
+                             void* workspace, size_t workspace_bytes, uwir_stream_t stream);
+
 /* ---- S/dwt_fft.py:61-72 fft2 / ifft2 (norm="ortho", full complex spectrum) ------------------
  * fwd: x [B,H,W,C] fp32 -> amp = |F|, phase = atan2(Im,Re) (both [B,H,W,C], stride ld_out).
  * inv: out = addend + Re(ifft2(amp*exp(i*phase)))  (S/sffb.py:52-54: spatial + freq).

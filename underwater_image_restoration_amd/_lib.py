@@ -80,6 +80,15 @@ _SIGS = {
     "uwir_flash_attn_workspace_bytes": (sz, [ci, ci, ci]),
     "uwir_flash_attn_packed_workspace_bytes": (sz, [ci, ci, ci, ci, ci]),
     "uwir_flash_attn": (ci, [vp, ci, vp, ci, vp, ci, vp, ci, ci, ci, ci, ci, ci, cf, vp, ci, vp, ci, ci, vp, sz, vp]),
+    "uwir_group_norm_act_workspace_bytes": (sz, [ci, ci, ci, ci]),
+    "uwir_group_norm_act": (ci, [vp, ci, sz, ci, ci, ci, ci, cf, vp, vp, vp, sz, ci, vp, ci, sz, vp, vp, vp, sz, vp]),
+    "uwir_group_norm_act_backward": (ci, [vp, sz, vp, sz, ci, ci, ci, ci, ci, vp, vp, vp, vp, vp, sz, ci, vp, sz, vp, vp, vp, sz,
+                                          vp, sz, vp]),
+    "uwir_cross_attn_workspace_bytes": (sz, [ci, ci, ci, ci, ci, ci, ci]),
+    "uwir_cross_attn": (ci, [vp, sz, vp, sz, vp, sz, ci, ci, ci, ci, ci, ci, ci, cf, vp, vp, sz, vp, sz, vp, vp, sz, vp]),
+    "uwir_cross_attn_backward_workspace_bytes": (sz, [ci, ci, ci, ci, ci, ci, ci]),
+    "uwir_cross_attn_backward": (ci, [vp, sz, vp, sz, vp, sz, vp, sz, vp, vp, sz, ci, ci, ci, ci, ci, ci, ci, cf, vp, vp, sz,
+                                      vp, sz, vp, sz, vp, sz, vp, sz, vp]),
     "uwir_fft_workspace_bytes": (sz, [ci, ci, ci, ci]),
     "uwir_fft2_amp_phase": (ci, [vp, ci, ci, ci, ci, ci, vp, vp, ci, vp, sz, vp]),
     "uwir_ifft2_polar_add": (ci, [vp, vp, ci, vp, ci, ci, ci, ci, ci, vp, ci, vp, sz, vp]),

@@ -13,7 +13,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libuwir_hip.so")
 SOURCES = ["elementwise.hip", "dwconv.hip", "gemm.hip", "gemm_wide.hip", "gemm_wide288.hip", "gate.hip", "ffn.hip", "attention.hip", "fft.hip", "tokens.hip", "unet.hip", "linattn.hip", "metrics.hip",
-           "teacher.hip", "enhance.hip", "enhance_cv.hip"]
+           "teacher.hip", "enhance.hip", "enhance_cv.hip", "groupnorm.hip", "cross_attn.hip",
+           "cross_attn_bwd.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # -amdgpu-mfma-vgpr-form: keep MFMA accumulators in VGPRs (gfx950 has a unified file); without it every softmax /
 # epilogue touch of an accumulator costs a v_accvgpr_read/write pair.
@@ -31,14 +32,14 @@ def _stale(target: str, deps) -> bool:
 def build(force: bool = False, verbose: bool = True) -> str:
     objdir = os.path.join(HERE, "build")
     os.makedirs(objdir, exist_ok=True)
-    headers = [os.path.join(CSRC, "common.h"), os.path.join(os.path.dirname(HERE), "include", "uwir.h")]
+    headers = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "cross_attn.h"), os.path.join(os.path.dirname(HERE), "include", "uwir.h")]
 
     def compile_one(src: str) -> str:
         s = os.path.join(CSRC, src)
         o = os.path.join(objdir, src.replace(".hip", ".o"))
         if force or _stale(o, [s] + headers + [os.path.abspath(__file__)]):
             # attention: fmaxf on MFMA outputs would otherwise get a canonicalising v_max per element
-            extra = ["-fno-honor-nans"] if src == "attention.hip" else []
+            extra = ["-fno-honor-nans"] if src in ("attention.hip", "cross_attn.hip", "cross_attn_bwd.hip") else []
             cmd = [HIPCC] + FLAGS + extra + ["-c", s, "-o", o]
             if verbose:
                 print(" ".join(cmd), flush=True)

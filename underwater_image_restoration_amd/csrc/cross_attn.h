@@ -1,0 +1,165 @@
+// Shared pieces of the cross-attention kernels (forward and backward).
+//
+// Everything is built on 32 x 32 accumulators of v_mfma_f32_32x32x16_bf16 / v_mfma_f32_32x32x2_f32, in which lane l holds
+// column l % 32 and rows (r & 3) + 8 (r >> 2) + 4 (l / 32), r = 0..15.  A product whose summed index lies on the rows of
+// such an accumulator takes it as its B operand straight from registers, as long as the A operand follows the same order
+// of the summed index; so probabilities and score gradients never pass through shared memory.  The two A operands:
+//   rows   row l % 32 of a row-major tile, 16 consecutive bytes a lane (K in K q^T, q in q K^T, ...)
+//   cols   column l % 32 of the same tile, summed rows in accumulator order (V^T P, K^T dS, q^T dS, dO^T P): one
+//          transposing LDS read per four rows (bf16), or plain reads (fp32, consecutive lanes = consecutive columns)
+#pragma once
+#include "common.h"
+
+namespace xattn {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.69314718055994531f;
+
+template <typename T> struct Mma;
+
+template <> struct Mma<bf16_t> {
+    static constexpr int VEC = 8, KSTEP = 16, PAD = 8;   // elements: per 16 bytes, per rows() step, of LDS row padding
+    typedef bf16x8 frag;
+    struct Prob { bf16x8 p[2]; };
+    static __device__ __forceinline__ void rows(f32x16& acc, frag a, frag b) {
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc, 0, 0, 0);
+    }
+    static __device__ __forceinline__ Prob pack(const float* v) {
+        Prob o;
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o.p[s][j] = (bf16_t)v[8 * s + j];
+        return o;
+    }
+    // acc[col0 + ., .] += tile[row0 .. row0 + 31][col0 + .]^T * prob.  Lane group of 16: four rows x 16 columns a read.
+    template <int STR> static __device__ __forceinline__ void cols(f32x16& acc, const bf16_t* tile, int lane, const Prob& b) {
+        typedef __attribute__((address_space(3))) bf16x4 lds4;
+        const bf16_t* p = tile + (4 * (lane >> 5) + ((lane & 15) >> 2)) * STR + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4*)(p + 16 * s * STR));
+            const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4*)(p + (16 * s + 8) * STR));
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), b.p[s], acc,
+                                                          0, 0, 0);
+        }
+    }
+};
+
+template <> struct Mma<float> {
+    static constexpr int VEC = 4, KSTEP = 8, PAD = 4;
+    typedef f32x4 frag;
+    struct Prob { float p[16]; };
+    static __device__ __forceinline__ void rows(f32x16& acc, frag a, frag b) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], acc, 0, 0, 0);
+    }
+    static __device__ __forceinline__ Prob pack(const float* v) {
+        Prob o;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o.p[r] = v[r];
+        return o;
+    }
+    template <int STR> static __device__ __forceinline__ void cols(f32x16& acc, const float* tile, int lane, const Prob& b) {
+        const float* p = tile + 4 * (lane >> 5) * STR + (lane & 31);
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            acc = __builtin_amdgcn_mfma_f32_32x32x2f32(p[((r & 3) + 8 * (r >> 2)) * STR], b.p[r], acc, 0, 0, 0);
+    }
+};
+
+__device__ __forceinline__ void zero16(f32x16& a) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) a[r] = 0.f;
+}
+
+// v of this lane and of lane ^ 32, in an order that depends on the half: for symmetric uses
+__device__ __forceinline__ float2 both_halves(float v) {
+    const unsigned u = __float_as_uint(v);
+    auto sw = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return make_float2(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+}
+
+// Accumulator rows 8q .. 8q+7 of a 32-row block (q = 0..3) sit as two quads, one in each half of the wave.  Swapping
+// quads between the halves leaves every lane with 8 consecutive rows: rows 16 t + 8 half + 0..7 for t = 0, 1.
+__device__ __forceinline__ void gather8(const f32x16& a, int t, float* o) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(a[8 * t + j]), __float_as_uint(a[8 * t + 4 + j]), false, false);
+        o[j] = __uint_as_float(sw[0]);
+        o[4 + j] = __uint_as_float(sw[1]);
+    }
+}
+
+__device__ __forceinline__ void store8(bf16_t* p, const float* v) {
+    bf16x8 o;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] = (bf16_t)v[j];
+    *reinterpret_cast<bf16x8*>(p) = o;
+}
+__device__ __forceinline__ void store8(float* p, const float* v) {
+    f32x4 a, b;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        a[j] = v[j];
+        b[j] = v[4 + j];
+    }
+    *reinterpret_cast<f32x4*>(p) = a;
+    *reinterpret_cast<f32x4*>(p + 4) = b;
+}
+
+// contiguous ranges of work per XCD (blocks are dealt to the 8 XCDs in turn): blocks that read the same keys share an L2
+__device__ __forceinline__ unsigned xcd_order(unsigned bid, unsigned nblocks) {
+    const unsigned q = nblocks / 8, r = nblocks % 8, x = bid % 8;
+    return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + bid / 8;
+}
+
+}  // namespace xattn
+
+// ---- host side: argument checks shared by both directions
+namespace {
+
+struct XMat {
+    const void* p;
+    size_t ld;
+    int heads;
+    size_t rows;
+    const char* name;
+};
+
+inline int xattn_check(const char* what, int dtype, int B, int nq, int nk, int heads, int kv_heads, int hd, float scale) {
+    UWIR_CHECK(dtype == UWIR_F32 || dtype == UWIR_BF16, "%s: bad dtype", what);
+    UWIR_CHECK(B > 0 && nq >= 0 && nk >= 0, "%s: bad shape (B > 0, nq >= 0, nk >= 0)", what);
+    UWIR_CHECK(heads > 0 && kv_heads > 0 && heads % kv_heads == 0, "%s: kv_heads must divide heads", what);
+    UWIR_CHECK((long long)B * kv_heads <= 65535 && (long long)nq * (heads / kv_heads) < (1ll << 30) && nk < (1 << 30),
+               "%s: too large (B * kv_heads <= 65535; nq * heads / kv_heads and nk below 2^30)", what);
+    UWIR_CHECK(hd > 0 && hd <= 128 && hd % 8 == 0, "%s: head size must be a multiple of 8, at most 128", what);
+    UWIR_CHECK(scale > 0.f && scale < 1e30f, "%s: scale must be positive and finite", what);
+    return UWIR_OK;
+}
+
+inline int xattn_check_mats(const char* what, int dtype, int hd, const XMat* in, int n_in, const XMat* out, int n_out) {
+    const size_t es = dtype == UWIR_BF16 ? 2 : 4;
+    auto bytes = [&](const XMat& m) { return m.rows ? ((m.rows - 1) * m.ld + (size_t)m.heads * hd) * es : 0; };
+    for (int i = 0; i < n_in + n_out; ++i) {
+        const XMat& m = i < n_in ? in[i] : out[i - n_in];
+        if (m.rows == 0) continue;
+        UWIR_CHECK(m.p, "%s: null pointer (%s)", what, m.name);
+        UWIR_CHECK(m.ld >= (size_t)m.heads * hd, "%s: row stride of %s is below heads * hd", what, m.name);
+        UWIR_CHECK(((uintptr_t)m.p & 15) == 0 && (m.ld * es) % 16 == 0, "%s: rows of %s must be 16-byte aligned", what, m.name);
+    }
+    // an output may share a wider matrix with another operand (column ranges that do not meet), but no element
+    for (int o = 0; o < n_out; ++o)
+        for (int i = 0; i < n_in + o; ++i) {
+            const XMat &a = out[o], &b = i < n_in ? in[i] : out[i - n_in];
+            const size_t na = bytes(a), nb = bytes(b), wa = (size_t)a.heads * hd * es, wb = (size_t)b.heads * hd * es;
+            const uintptr_t x = (uintptr_t)a.p, y = (uintptr_t)b.p;
+            if (!na || !nb || x + na <= y || y + nb <= x) continue;
+            const size_t ld = a.ld * es;
+            const size_t d = x >= y ? (x - y) % ld : (ld - (y - x) % ld) % ld;   // a's first column, seen from b's
+            UWIR_CHECK(a.ld == b.ld && d >= wb && d + wa <= ld, "%s: %s overlaps %s", what, a.name, b.name);
+        }
+    return UWIR_OK;
+}
+
+}  // namespace

@@ -1,0 +1,563 @@
+// Cross attention, backward.  With s = scale q k^T over the visible keys and p = exp(s - lse):
+//   D = sum_d dout out,  dv = p^T dout,  dp = dout v^T,  ds = p (dp - D),  dq = scale ds k,  dk = scale ds^T q
+// Two kernels, each of which keeps its result in registers and forms p again (7 products instead of the 5 that one kernel
+// with both results would need; in exchange nothing is accumulated through memory in an order that changes):
+//   rows kernel  a wave owns 32 packed rows (cross_attn.hip), walks the keys: S^T = K q^T, dP^T = V dout^T,
+//                dq^T += K^T dS; also forms D and hands (lse, D) to the next kernel in packed-row order
+//   keys kernel  a wave owns 32 keys, walks the rows of all query heads that share them: S = q K^T, dP = dout V^T,
+//                dv^T += dout^T P, dk^T += q^T dS -- the sum over shared heads and rows never leaves the registers
+// Either splits its long axis over blocks when there are few; the parts (fp32) are then summed in order by a last launch.
+#include "cross_attn.h"
+
+using namespace xattn;
+
+namespace {
+
+struct BArgs {
+    const void *q, *k, *v, *o, *go;
+    const float* lse;
+    void *dq, *dk, *dv;
+    const int* lens;
+    const unsigned char* mask;
+    float2* ld;                    // [B * KV][R] (lse in the log2 domain, D)
+    float *part_q, *part_k, *part_v;
+    size_t ldq, ldk, ldv, ldo, ldg, ld_dq, ld_dk, ld_dv, ldm;
+    int B, nq, nk, H, KV, hd, G, R;
+    int qsplits, qtiles, qblocks;  // rows kernel
+    int ksplits, ktiles, kblocks;  // keys kernel
+    float c, scale;
+};
+
+template <typename T, int HD> struct Tile {
+    typedef Mma<T> M;
+    static constexpr int VEC = M::VEC, STR = HD + M::PAD, CPR = HD / VEC;
+};
+
+struct RowRef {
+    size_t row;
+    int head;
+};
+__device__ __forceinline__ RowRef row_ref(const BArgs& p, int b, int kv, int r) {
+    const int qi = p.G == 1 ? r : r / p.G;
+    return {(size_t)b * p.nq + qi, kv * p.G + (r - qi * p.G)};
+}
+
+__device__ __forceinline__ int image_len(const BArgs& p, int b) {
+    return p.lens ? max(0, min(p.nk, p.lens[b])) : p.nk;
+}
+
+template <typename F> __device__ __forceinline__ F zero_frag() {
+    F f;
+#pragma unroll
+    for (int j = 0; j < (int)(sizeof(F) / sizeof(f[0])); ++j) f[j] = 0;
+    return f;
+}
+
+// ---------------------------------------------------------------------------------------- dq
+template <typename T, int HD, int QG>
+__global__ void __launch_bounds__(256) xattn_dq_kernel(BArgs p) {
+    typedef Tile<T, HD> L;
+    typedef typename L::M M;
+    typedef typename M::frag frag;
+    constexpr int KT = 64, NC = KT * L::CPR / 256, KS = HD / M::KSTEP, DG = HD / 32;
+    __shared__ __attribute__((aligned(16))) T sK[2][KT * L::STR];
+    __shared__ __attribute__((aligned(16))) T sV[2][KT * L::STR];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const unsigned vid = xcd_order(blockIdx.x, p.qblocks);
+    const int qt = vid % p.qtiles, split = (vid / p.qtiles) % p.qsplits, bk = vid / p.qtiles / p.qsplits;
+    const int b = bk / p.KV, kv = bk % p.KV;
+    int begin = 0, end = image_len(p, b);
+    if (p.qsplits > 1) {
+        const int tiles = (end + KT - 1) / KT, per = (tiles + p.qsplits - 1) / p.qsplits;
+        begin = min(end, split * per * KT);
+        end = min(end, (split + 1) * per * KT);
+    }
+    const T* K = (const T*)p.k + (size_t)b * p.nk * p.ldk + (size_t)kv * p.hd;
+    const T* V = (const T*)p.v + (size_t)b * p.nk * p.ldv + (size_t)kv * p.hd;
+    const unsigned char* mask = p.mask ? p.mask + (size_t)b * p.ldm : nullptr;
+
+    frag rk[NC], rv[NC];
+    bool vis;
+    auto load = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            const int ci = tid + 256 * i, d = (ci % L::CPR) * L::VEC, key = min(k0 + ci / L::CPR, end - 1);
+            rk[i] = rv[i] = zero_frag<frag>();
+            if (d < p.hd) {
+                rk[i] = *reinterpret_cast<const frag*>(K + (size_t)key * p.ldk + d);
+                rv[i] = *reinterpret_cast<const frag*>(V + (size_t)key * p.ldv + d);
+            }
+        }
+        vis = k0 + lane < end && (!mask || mask[k0 + lane]);
+    };
+    auto store = [&](int buf, unsigned long long bits) {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            const int ci = tid + 256 * i, row = ci / L::CPR, d = (ci % L::CPR) * L::VEC;
+            if (bits != ~0ull && !((bits >> row) & 1)) rk[i] = rv[i] = zero_frag<frag>();   // whatever hidden keys hold
+            *reinterpret_cast<frag*>(&sK[buf][row * L::STR + d]) = rk[i];
+            *reinterpret_cast<frag*>(&sV[buf][row * L::STR + d]) = rv[i];
+        }
+    };
+
+    frag fq[QG][KS], fg[QG][KS];
+    f32x16 dq[QG][DG];
+    float l2[QG], D[QG];
+    const int row0 = (qt * 4 + wave) * 32 * QG + (lane & 31);
+#pragma unroll
+    for (int g = 0; g < QG; ++g) {
+        const int r = row0 + 32 * g;
+        const bool ok = r < p.R;
+        const RowRef f = row_ref(p, b, kv, ok ? r : 0);
+        const T* Q = (const T*)p.q + f.row * p.ldq + (size_t)f.head * p.hd;
+        const T* GO = (const T*)p.go + f.row * p.ldg + (size_t)f.head * p.hd;
+        const T* O = (const T*)p.o + f.row * p.ldo + (size_t)f.head * p.hd;
+        float dd = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const int d = ks * M::KSTEP + (lane >> 5) * M::VEC;
+            fq[g][ks] = fg[g][ks] = zero_frag<frag>();
+            if (ok && d < p.hd) {
+                fq[g][ks] = *reinterpret_cast<const frag*>(Q + d);
+                fg[g][ks] = *reinterpret_cast<const frag*>(GO + d);
+                const frag o = *reinterpret_cast<const frag*>(O + d);
+#pragma unroll
+                for (int j = 0; j < M::VEC; ++j) dd = fmaf((float)fg[g][ks][j], (float)o[j], dd);
+            }
+        }
+        const float2 h = both_halves(dd);
+        D[g] = h.x + h.y;
+        float l = ok ? p.lse[((size_t)b * p.H + f.head) * p.nq + (f.row - (size_t)b * p.nq)] * LOG2E : 0.f;
+        l2[g] = l == -INFINITY ? 0.f : l;   // an image that shows nothing: no tile below has a visible key
+        if (ok && split == 0 && lane < 32) p.ld[(size_t)bk * p.R + r] = make_float2(l2[g], D[g]);
+#pragma unroll
+        for (int dg = 0; dg < DG; ++dg) zero16(dq[g][dg]);
+    }
+    const float c = p.c;
+    const bool idle = (qt * 4 + wave) * 32 * QG >= p.R;
+
+    unsigned long long bits = 0;
+    if (begin < end) {
+        load(begin);
+        bits = __ballot(vis);
+        store(0, bits);
+    }
+    __syncthreads();
+    int buf = 0;
+    for (int k0 = begin; k0 < end; k0 += KT, buf ^= 1) {
+        const bool more = k0 + KT < end;
+        if (more) load(k0 + KT);
+        if (bits && !idle) {
+#pragma unroll
+            for (int kb = 0; kb < KT / 32; ++kb) {
+                const unsigned b32 = (unsigned)(bits >> (32 * kb));
+                if (!b32) continue;
+                f32x16 s[QG], dp[QG];
+#pragma unroll
+                for (int g = 0; g < QG; ++g) {
+                    zero16(s[g]);
+                    zero16(dp[g]);
+                }
+                const int off = (32 * kb + (lane & 31)) * L::STR + (lane >> 5) * L::VEC;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    const frag kf = *reinterpret_cast<const frag*>(&sK[buf][off + ks * M::KSTEP]);
+                    const frag vf = *reinterpret_cast<const frag*>(&sV[buf][off + ks * M::KSTEP]);
+#pragma unroll
+                    for (int g = 0; g < QG; ++g) {
+                        M::rows(s[g], kf, fq[g][ks]);
+                        M::rows(dp[g], vf, fg[g][ks]);
+                    }
+                }
+                typename M::Prob ds[QG];
+                const unsigned hb = b32 >> (4 * (lane >> 5));
+#pragma unroll
+                for (int g = 0; g < QG; ++g) {
+                    float v[16];
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        v[r] = __builtin_amdgcn_exp2f(fmaf(s[g][r], c, -l2[g])) * (dp[g][r] - D[g]);
+                        if (b32 != ~0u) v[r] = (hb >> ((r & 3) + 8 * (r >> 2))) & 1u ? v[r] : 0.f;
+                    }
+                    ds[g] = M::pack(v);
+                }
+#pragma unroll
+                for (int dg = 0; dg < DG; ++dg)
+#pragma unroll
+                    for (int g = 0; g < QG; ++g)
+                        M::template cols<L::STR>(dq[g][dg], &sK[buf][32 * kb * L::STR + 32 * dg], lane, ds[g]);
+            }
+        }
+        if (more) {
+            bits = __ballot(vis);
+            store(buf ^ 1, bits);
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int g = 0; g < QG; ++g) {
+        const int r = row0 + 32 * g;
+        if (r >= p.R) continue;
+        const RowRef f = row_ref(p, b, kv, r);
+        T* dst = (T*)p.dq + f.row * p.ld_dq + (size_t)f.head * p.hd;
+        float* part = p.part_q + (((size_t)split * p.B * p.KV + bk) * p.R + r) * p.hd;
+#pragma unroll
+        for (int dg = 0; dg < DG; ++dg)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                float v[8];
+                gather8(dq[g][dg], t, v);
+                const int d = 32 * dg + 16 * t + 8 * (lane >> 5);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] *= p.scale;
+                if (d < p.hd) {
+                    if (p.qsplits > 1) store8(part + d, v);
+                    else store8(dst + d, v);
+                }
+            }
+    }
+}
+
+// ---------------------------------------------------------------------------------------- dk, dv
+// KW waves across the keys (32 each); the 4 / KW waves of one key group take the 32-row blocks of a tile in turn
+template <typename T, int HD, int KW>
+__global__ void __launch_bounds__(256) xattn_dkv_kernel(BArgs p) {
+    typedef Tile<T, HD> L;
+    typedef typename L::M M;
+    typedef typename M::frag frag;
+    constexpr int WR = 4 / KW, RT = 32 * (WR > 2 ? WR : 2), NC = RT * L::CPR / 256, KS = HD / M::KSTEP, DG = HD / 32;
+    constexpr int TILE = RT * L::STR, JSTR = HD + 1;
+    constexpr size_t LOOP = (size_t)4 * TILE * sizeof(T), JOIN = WR > 1 ? (size_t)4 * 32 * JSTR * 4 : 0;
+    __shared__ __attribute__((aligned(16))) char smem[LOOP > JOIN ? LOOP : JOIN];
+    __shared__ __attribute__((aligned(16))) float sL[2][RT], sD[2][RT];
+    T* sQ = reinterpret_cast<T*>(smem);            // [2][TILE]
+    T* sG = sQ + 2 * TILE;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, kw = wave % KW, wr = wave / KW;
+    const unsigned vid = xcd_order(blockIdx.x, p.kblocks);
+    const int kt = vid % p.ktiles, split = (vid / p.ktiles) % p.ksplits, bk = vid / p.ktiles / p.ksplits;
+    const int b = bk / p.KV, kv = bk % p.KV;
+    const int len = image_len(p, b), key0 = kt * 32 * KW, key = key0 + 32 * kw + (lane & 31);
+    const bool vis = key < len && (!p.mask || p.mask[(size_t)b * p.ldm + key]);
+
+    frag fk[KS], fv[KS];
+    f32x16 dk[DG], dv[DG];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        const int d = ks * M::KSTEP + (lane >> 5) * M::VEC;
+        fk[ks] = fv[ks] = zero_frag<frag>();
+        if (vis && d < p.hd) {
+            fk[ks] = *reinterpret_cast<const frag*>((const T*)p.k + ((size_t)b * p.nk + key) * p.ldk + (size_t)kv * p.hd + d);
+            fv[ks] = *reinterpret_cast<const frag*>((const T*)p.v + ((size_t)b * p.nk + key) * p.ldv + (size_t)kv * p.hd + d);
+        }
+    }
+#pragma unroll
+    for (int dg = 0; dg < DG; ++dg) {
+        zero16(dk[dg]);
+        zero16(dv[dg]);
+    }
+    int begin = 0, end = p.R;
+    if (p.ksplits > 1) {
+        const int tiles = (p.R + RT - 1) / RT, per = (tiles + p.ksplits - 1) / p.ksplits;
+        begin = min(p.R, split * per * RT);
+        end = min(p.R, (split + 1) * per * RT);
+    }
+    // a block whose keys are all hidden has nothing to add up (block-uniform, ahead of every barrier but this one)
+    if (!__syncthreads_or(vis)) end = begin;
+    const bool idle = !__any(vis);
+
+    frag rq[NC], rg[NC];
+    float2 rl;
+    auto load = [&](int r0) {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            const int ci = tid + 256 * i, d = (ci % L::CPR) * L::VEC, r = r0 + ci / L::CPR;
+            rq[i] = rg[i] = zero_frag<frag>();
+            if (r < end && d < p.hd) {
+                const RowRef f = row_ref(p, b, kv, r);
+                rq[i] = *reinterpret_cast<const frag*>((const T*)p.q + f.row * p.ldq + (size_t)f.head * p.hd + d);
+                rg[i] = *reinterpret_cast<const frag*>((const T*)p.go + f.row * p.ldg + (size_t)f.head * p.hd + d);
+            }
+        }
+        rl = make_float2(0.f, 0.f);
+        if (tid < RT && r0 + tid < end) rl = p.ld[(size_t)bk * p.R + r0 + tid];
+    };
+    auto store = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            const int ci = tid + 256 * i, row = ci / L::CPR, d = (ci % L::CPR) * L::VEC;
+            *reinterpret_cast<frag*>(&sQ[buf * TILE + row * L::STR + d]) = rq[i];
+            *reinterpret_cast<frag*>(&sG[buf * TILE + row * L::STR + d]) = rg[i];
+        }
+        if (tid < RT) {
+            sL[buf][tid] = rl.x;
+            sD[buf][tid] = rl.y;
+        }
+    };
+    const float c = p.c;
+    if (begin < end) {
+        load(begin);
+        store(0);
+    }
+    __syncthreads();
+    int buf = 0;
+    for (int r0 = begin; r0 < end; r0 += RT, buf ^= 1) {
+        const bool more = r0 + RT < end;
+        if (more) load(r0 + RT);
+        if (!idle) {
+#pragma unroll
+            for (int i = 0; i < RT / 32 / WR; ++i) {
+                const int rb = WR == 1 ? i : i * WR + wr;
+                const T* tq = sQ + buf * TILE + 32 * rb * L::STR;
+                const T* tg = sG + buf * TILE + 32 * rb * L::STR;
+                const int off = (lane & 31) * L::STR + (lane >> 5) * L::VEC;
+                f32x16 s, dp;
+                zero16(s);
+                zero16(dp);
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    M::rows(s, *reinterpret_cast<const frag*>(tq + off + ks * M::KSTEP), fk[ks]);
+                    M::rows(dp, *reinterpret_cast<const frag*>(tg + off + ks * M::KSTEP), fv[ks]);
+                }
+                float pr[16], ds[16];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const f32x4 l = *reinterpret_cast<const f32x4*>(&sL[buf][32 * rb + 8 * u + 4 * (lane >> 5)]);
+                    const f32x4 D = *reinterpret_cast<const f32x4*>(&sD[buf][32 * rb + 8 * u + 4 * (lane >> 5)]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float e = __builtin_amdgcn_exp2f(fmaf(s[4 * u + j], c, -l[j]));
+                        pr[4 * u + j] = vis ? e : 0.f;
+                        ds[4 * u + j] = pr[4 * u + j] * (dp[4 * u + j] - D[j]);
+                    }
+                }
+                const typename M::Prob pp = M::pack(pr), pd = M::pack(ds);
+#pragma unroll
+                for (int dg = 0; dg < DG; ++dg) {
+                    M::template cols<L::STR>(dv[dg], tg + 32 * dg, lane, pp);
+                    M::template cols<L::STR>(dk[dg], tq + 32 * dg, lane, pd);
+                }
+            }
+        }
+        if (more) store(buf ^ 1);
+        __syncthreads();
+    }
+    if constexpr (WR > 1) {   // join the row waves of each key group, dk first, then dv
+        float* sj = reinterpret_cast<float*>(smem);
+        auto join = [&](f32x16* a) {
+#pragma unroll
+            for (int dg = 0; dg < DG; ++dg)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    sj[(wave * 32 + (lane & 31)) * JSTR + 32 * dg + (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5)] = a[dg][r];
+            __syncthreads();
+#pragma unroll
+            for (int dg = 0; dg < DG; ++dg)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    float t = 0.f;
+#pragma unroll
+                    for (int w = 0; w < WR; ++w)
+                        t += sj[((w * KW + kw) * 32 + (lane & 31)) * JSTR + 32 * dg + (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5)];
+                    a[dg][r] = t;
+                }
+            __syncthreads();
+        };
+        join(dk);
+        join(dv);
+        if (wr != 0) return;
+    }
+    if (key >= p.nk) return;
+    const size_t row = (size_t)b * p.nk + key;
+    T* ok = (T*)p.dk + row * p.ld_dk + (size_t)kv * p.hd;
+    T* ov = (T*)p.dv + row * p.ld_dv + (size_t)kv * p.hd;
+    const size_t po = (((size_t)split * p.B * p.nk + row) * p.KV + kv) * p.hd;
+#pragma unroll
+    for (int dg = 0; dg < DG; ++dg)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            float a[8], v[8];
+            gather8(dk[dg], t, a);
+            gather8(dv[dg], t, v);
+            const int d = 32 * dg + 16 * t + 8 * (lane >> 5);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) a[j] = vis ? a[j] * p.scale : 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = vis ? v[j] : 0.f;
+            if (d < p.hd) {
+                if (p.ksplits > 1) {
+                    store8(p.part_k + po + d, a);
+                    store8(p.part_v + po + d, v);
+                } else {
+                    store8(ok + d, a);
+                    store8(ov + d, v);
+                }
+            }
+        }
+}
+
+// out[row][d] = sum over the parts, in order; one thread per row, head and 8 columns.  grid.y: 0 = dk, 1 = dv
+template <typename T>
+__global__ void __launch_bounds__(256) xattn_sum_keys_kernel(BArgs p) {
+    const int cpr = p.KV * p.hd / 8;
+    const size_t rows = (size_t)p.B * p.nk, i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= rows * cpr) return;
+    const size_t row = i / cpr, d = 8 * (i % cpr), stride = rows * p.KV * p.hd;
+    const float* src = (blockIdx.y ? p.part_v : p.part_k) + row * p.KV * p.hd + d;
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = 0.f;
+    for (int s = 0; s < p.ksplits; ++s) {
+        const f32x4 a = *reinterpret_cast<const f32x4*>(src + s * stride), e = *reinterpret_cast<const f32x4*>(src + s * stride + 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            v[j] += a[j];
+            v[4 + j] += e[j];
+        }
+    }
+    store8(blockIdx.y ? (T*)p.dv + row * p.ld_dv + d : (T*)p.dk + row * p.ld_dk + d, v);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) xattn_sum_rows_kernel(BArgs p) {
+    const int cpr = p.hd / 8;
+    const size_t rows = (size_t)p.B * p.KV * p.R, i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= rows * cpr) return;
+    const size_t pr = i / cpr;
+    const int d = 8 * (int)(i % cpr);
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = 0.f;
+    for (int s = 0; s < p.qsplits; ++s) {
+        const float* src = p.part_q + (s * rows + pr) * p.hd + d;
+        const f32x4 a = *reinterpret_cast<const f32x4*>(src), e = *reinterpret_cast<const f32x4*>(src + 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            v[j] += a[j];
+            v[4 + j] += e[j];
+        }
+    }
+    const int r = (int)(pr % p.R), kv = (int)(pr / p.R % p.KV), b = (int)(pr / p.R / p.KV);
+    const RowRef f = row_ref(p, b, kv, r);
+    store8((T*)p.dq + f.row * p.ld_dq + (size_t)f.head * p.hd + d, v);
+}
+
+// ---------------------------------------------------------------------------------------- launch rules
+struct Plan {
+    int qsplits, qtiles, kw, ksplits, ktiles;
+};
+
+int hd_class(int hd) { return hd <= 32 ? 32 : hd <= 64 ? 64 : 128; }
+
+// parts of an axis of `tiles` steps so that `blocks` blocks grow to about two per CU, each with two steps at least
+int parts(long long blocks, long long tiles) {
+    long long s = blocks >= 384 ? 1 : (512 + blocks - 1) / (blocks > 0 ? blocks : 1);
+    if (s > tiles / 2) s = tiles / 2;
+    if (s > 64) s = 64;
+    return s < 1 ? 1 : (int)s;
+}
+
+Plan plan_bwd(int B, int nq, int nk, int H, int KV, int hd, int dtype) {
+    Plan pl = {};
+    const long long R = (long long)nq * (H / KV), bk = (long long)B * KV;
+    pl.qtiles = (int)((R + 127) / 128);
+    pl.qsplits = parts(bk * pl.qtiles, (nk + 63) / 64);
+    // few keys: waves beyond them take rows instead (fp32 rows of 128 columns leave no LDS for the longer row tiles)
+    pl.kw = hd > 64 && dtype == UWIR_F32 ? 4 : nk <= 32 ? 1 : nk <= 64 ? 2 : 4;
+    pl.ktiles = (nk + 32 * pl.kw - 1) / (32 * pl.kw);
+    pl.ksplits = parts(bk * pl.ktiles, (R + 63) / 64);
+    return pl;
+}
+
+size_t al256(size_t v) { return (v + 255) & ~(size_t)255; }
+
+struct Layout {
+    size_t ld, q, k, v, total;
+};
+Layout layout(const Plan& pl, int B, int nq, int nk, int H, int KV, int hd) {
+    Layout l;
+    size_t at = al256((size_t)B * H * nq * sizeof(float2));
+    l.ld = 0;
+    l.q = at;
+    if (pl.qsplits > 1) at += al256((size_t)pl.qsplits * B * H * nq * hd * 4);
+    l.k = at;
+    if (pl.ksplits > 1) at += al256((size_t)pl.ksplits * B * nk * KV * hd * 4);
+    l.v = at;
+    if (pl.ksplits > 1) at += al256((size_t)pl.ksplits * B * nk * KV * hd * 4);
+    l.total = at;
+    return l;
+}
+
+template <typename T, int HD> void launch(const BArgs& p, const Plan& pl, hipStream_t st) {
+    if (p.nq > 0) {
+        hipLaunchKernelGGL((xattn_dq_kernel<T, HD, 1>), dim3(p.qblocks), dim3(256), 0, st, p);
+        if (p.qsplits > 1) {
+            const size_t n = (size_t)p.B * p.KV * p.R * (p.hd / 8);
+            hipLaunchKernelGGL((xattn_sum_rows_kernel<T>), dim3((unsigned)ceil_div_sz(n, 256)), dim3(256), 0, st, p);
+        }
+    }
+    if (p.nk > 0) {
+        if constexpr (sizeof(T) == 2 || HD <= 64) {
+            if (pl.kw == 1) hipLaunchKernelGGL((xattn_dkv_kernel<T, HD, 1>), dim3(p.kblocks), dim3(256), 0, st, p);
+            if (pl.kw == 2) hipLaunchKernelGGL((xattn_dkv_kernel<T, HD, 2>), dim3(p.kblocks), dim3(256), 0, st, p);
+        }
+        if (pl.kw == 4) hipLaunchKernelGGL((xattn_dkv_kernel<T, HD, 4>), dim3(p.kblocks), dim3(256), 0, st, p);
+        if (p.ksplits > 1) {
+            const size_t n = (size_t)p.B * p.nk * p.KV * (p.hd / 8);
+            hipLaunchKernelGGL((xattn_sum_keys_kernel<T>), dim3((unsigned)ceil_div_sz(n, 256), 2), dim3(256), 0, st, p);
+        }
+    }
+}
+
+}  // namespace
+
+extern "C" size_t uwir_cross_attn_backward_workspace_bytes(int B, int nq, int nk, int heads, int kv_heads, int hd, int dtype) {
+    if (B <= 0 || nq < 0 || nk < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || hd <= 0) return 0;
+    return layout(plan_bwd(B, nq, nk, heads, kv_heads, hd, dtype), B, nq, nk, heads, kv_heads, hd).total;
+}
+
+extern "C" int uwir_cross_attn_backward(const void* q, size_t ldq, const void* k, size_t ldk, const void* v, size_t ldv,
+                                        const void* out, size_t ldo, const float* lse, const void* dout, size_t ld_dout, int dtype,
+                                        int B, int nq, int nk, int heads, int kv_heads, int hd, float scale, const int* key_lens,
+                                        const unsigned char* key_mask, size_t ld_mask, void* dq, size_t ld_dq, void* dk,
+                                        size_t ld_dk, void* dv, size_t ld_dv, void* workspace, size_t workspace_bytes,
+                                        uwir_stream_t stream) {
+    if (int rc = xattn_check("cross_attn_backward", dtype, B, nq, nk, heads, kv_heads, hd, scale)) return rc;
+    if (nq == 0 && nk == 0) return UWIR_OK;
+    const size_t rq = (size_t)B * nq, rk = (size_t)B * nk;
+    const XMat in[] = {{q, ldq, heads, rq, "q"}, {k, ldk, kv_heads, rk, "k"}, {v, ldv, kv_heads, rk, "v"}, {out, ldo, heads, rq, "out"},
+                       {dout, ld_dout, heads, rq, "dout"}};
+    const XMat res[] = {{dq, ld_dq, heads, rq, "dq"}, {dk, ld_dk, kv_heads, rk, "dk"}, {dv, ld_dv, kv_heads, rk, "dv"}};
+    if (int rc = xattn_check_mats("cross_attn_backward", dtype, hd, in, 5, res, 3)) return rc;
+    UWIR_CHECK(nq == 0 || lse, "cross_attn_backward: null pointer (lse)");
+    UWIR_CHECK(!key_mask || ld_mask >= (size_t)nk, "cross_attn_backward: mask rows must have at least nk entries");
+    const size_t need = uwir_cross_attn_backward_workspace_bytes(B, nq, nk, heads, kv_heads, hd, dtype);
+    UWIR_CHECK(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
+               "cross_attn_backward: workspace too small or not 16-byte aligned");
+    const Plan pl = plan_bwd(B, nq, nk, heads, kv_heads, hd, dtype);
+    const Layout lo = layout(pl, B, nq, nk, heads, kv_heads, hd);
+    BArgs p = {};
+    p.q = q; p.k = k; p.v = v; p.o = out; p.go = dout; p.lse = lse; p.dq = dq; p.dk = dk; p.dv = dv;
+    p.lens = key_lens; p.mask = key_mask;
+    p.ldq = ldq; p.ldk = ldk; p.ldv = ldv; p.ldo = ldo; p.ldg = ld_dout; p.ld_dq = ld_dq; p.ld_dk = ld_dk; p.ld_dv = ld_dv;
+    p.ldm = ld_mask;
+    p.B = B; p.nq = nq; p.nk = nk; p.H = heads; p.KV = kv_heads; p.hd = hd; p.G = heads / kv_heads; p.R = nq * p.G;
+    p.qsplits = pl.qsplits; p.qtiles = pl.qtiles; p.ksplits = pl.ksplits; p.ktiles = pl.ktiles;
+    const long long qb = (long long)B * kv_heads * pl.qtiles * pl.qsplits, kb = (long long)B * kv_heads * pl.ktiles * pl.ksplits;
+    UWIR_CHECK(qb < (1ll << 31) && kb < (1ll << 31), "cross_attn_backward: too many rows for one launch");
+    p.qblocks = (int)qb; p.kblocks = (int)kb;
+    p.c = scale * LOG2E; p.scale = scale;
+    char* ws = (char*)workspace;
+    p.ld = (float2*)(ws + lo.ld);
+    p.part_q = (float*)(ws + lo.q); p.part_k = (float*)(ws + lo.k); p.part_v = (float*)(ws + lo.v);
+    hipStream_t st = (hipStream_t)stream;
+    switch (hd_class(hd) + (dtype == UWIR_BF16)) {
+        case 32: launch<float, 32>(p, pl, st); break;
+        case 33: launch<bf16_t, 32>(p, pl, st); break;
+        case 64: launch<float, 64>(p, pl, st); break;
+        case 65: launch<bf16_t, 64>(p, pl, st); break;
+        case 128: launch<float, 128>(p, pl, st); break;
+        default: launch<bf16_t, 128>(p, pl, st); break;
+    }
+    UWIR_LAUNCH_CHECK("cross_attn_backward");
+    return UWIR_OK;
+}

@@ -347,6 +347,159 @@ def flash_attn(q, k, v1, v2, B: int, n: int, heads: int, hd: int, scale: float, 
         _TIMING["events"].append((("flash_attn", B, n, heads, hd, 1 if v2 is None else 2, dt), ev0, ev1))
 
 
+def _operands(what: str, first: torch.Tensor, *ts) -> None:
+    """Every given tensor on one GPU: a kernel follows raw pointers, whatever device they belong to."""
+    for t in ts:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{what}: operands on {first.device} and {t.device}")
+
+
+def _rows_cols(what: str, name: str, t: torch.Tensor, rows: int, cols: int) -> None:
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols or (t.stride(1) != 1 and cols > 1):
+        raise ValueError(f"{what}: {name} must be a [{rows}, {cols}] view with unit inner stride, got {tuple(t.shape)}")
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    """Row stride of a 2-D view; of a single row (whose stride means nothing) its width."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+
+
+def _vector(what: str, name: str, t: Optional[torch.Tensor], *shape) -> None:
+    if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous()):
+        raise ValueError(f"{what}: {name} must be a contiguous fp32 {list(shape)}")
+
+
+def group_norm_act_workspace_bytes(B: int, n: int, C_: int, groups: int) -> int:
+    return int(_lib.load().uwir_group_norm_act_workspace_bytes(B, n, C_, groups))
+
+
+def _gn_check(what, x, B, n, C_, groups, gamma, beta, act, scale_shift, workspace):
+    if B < 1 or n < 1 or C_ < 1 or groups < 1 or C_ % groups:
+        raise ValueError(f"{what}: need B, n, C > 0 and groups dividing C")
+    if act not in (ACT_NONE, ACT_SILU):
+        raise ValueError(f"{what}: act must be ACT_NONE or ACT_SILU")
+    _rows_cols(what, "x", x, B * n, C_)
+    _vector(what, "gamma", gamma, C_)
+    _vector(what, "beta", beta, C_)
+    if scale_shift is not None:
+        _f32(scale_shift)
+        _rows_cols(what, "scale_shift", scale_shift, B, 2 * C_)
+    if not workspace.is_contiguous():
+        raise ValueError(f"{what}: workspace must be contiguous")
+
+
+def group_norm_act(x: torch.Tensor, B: int, n: int, C_: int, groups: int, eps: float, gamma: torch.Tensor, beta: torch.Tensor,
+                   out: torch.Tensor, workspace: torch.Tensor, act: int = ACT_NONE, scale_shift: Optional[torch.Tensor] = None,
+                   mean: Optional[torch.Tensor] = None, rstd: Optional[torch.Tensor] = None) -> None:
+    """out = act((GroupNorm(x) gamma + beta) (1 + scale_b) + shift_b) on NHWC rows x, out [B * n, C] (fp32 / bf16 each; out may
+    be x).  ``scale_shift`` [B, 2C] = [scale | shift] per image.  ``mean`` / ``rstd`` [B, groups] keep the statistics for
+    ``group_norm_act_backward``.  workspace: group_norm_act_workspace_bytes, any contiguous tensor; see uwir_group_norm_act."""
+    what = "group_norm_act"
+    _gn_check(what, x, B, n, C_, groups, gamma, beta, act, scale_shift, workspace)
+    _rows_cols(what, "out", out, B * n, C_)
+    _vector(what, "mean", mean, B, groups)
+    _vector(what, "rstd", rstd, B, groups)
+    _operands(what, x, gamma, beta, out, workspace, scale_shift, mean, rstd)
+    _lib.check(_lib.load().uwir_group_norm_act(
+        _p(x), _dt(x), _row_stride(x), B, n, C_, groups, eps, _p(gamma), _p(beta), _p(scale_shift),
+        0 if scale_shift is None else _row_stride(scale_shift), act, _p(out), _dt(out), _row_stride(out), _p(mean), _p(rstd),
+        _p(workspace), workspace.numel() * workspace.element_size(), _stream(x)), what)
+
+
+def group_norm_act_backward(dy: torch.Tensor, x: torch.Tensor, B: int, n: int, C_: int, groups: int, gamma: torch.Tensor,
+                            beta: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, dx: torch.Tensor, dgamma: torch.Tensor,
+                            dbeta: torch.Tensor, workspace: torch.Tensor, act: int = ACT_NONE,
+                            scale_shift: Optional[torch.Tensor] = None, dscale_shift: Optional[torch.Tensor] = None) -> None:
+    """Gradients of ``group_norm_act``: dx [B * n, C] (dtype of x and dy; may be either of them), dgamma, dbeta [C] fp32 and
+    dscale_shift [B, 2C] fp32 (written, not added to) from the forward call's x, mean and rstd."""
+    what = "group_norm_act_backward"
+    _gn_check(what, x, B, n, C_, groups, gamma, beta, act, scale_shift, workspace)
+    _rows_cols(what, "dy", dy, B * n, C_)
+    _rows_cols(what, "dx", dx, B * n, C_)
+    if dy.dtype != x.dtype or dx.dtype != x.dtype:
+        raise TypeError(f"{what}: x, dy and dx must share a dtype")
+    for name, t, shape in (("mean", mean, (B, groups)), ("rstd", rstd, (B, groups)), ("dgamma", dgamma, (C_,)), ("dbeta", dbeta, (C_,))):
+        _vector(what, name, t, *shape)
+    if dscale_shift is not None:
+        if scale_shift is None:
+            raise ValueError(f"{what}: dscale_shift without scale_shift")
+        _f32(dscale_shift)
+        _rows_cols(what, "dscale_shift", dscale_shift, B, 2 * C_)
+    _operands(what, x, dy, gamma, beta, mean, rstd, dx, dgamma, dbeta, workspace, scale_shift, dscale_shift)
+    _lib.check(_lib.load().uwir_group_norm_act_backward(
+        _p(dy), _row_stride(dy), _p(x), _row_stride(x), _dt(x), B, n, C_, groups, _p(gamma), _p(beta), _p(mean), _p(rstd),
+        _p(scale_shift), 0 if scale_shift is None else _row_stride(scale_shift), act, _p(dx), _row_stride(dx), _p(dgamma),
+        _p(dbeta), _p(dscale_shift), 0 if dscale_shift is None else _row_stride(dscale_shift), _p(workspace),
+        workspace.numel() * workspace.element_size(), _stream(x)), what)
+
+
+def _torch_dt(dtype: torch.dtype) -> int:
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"unsupported dtype {dtype}")
+    return F32 if dtype == torch.float32 else BF16
+
+
+def cross_attn_workspace_bytes(B: int, nq: int, nk: int, heads: int, kv_heads: int, hd: int, dtype: torch.dtype) -> int:
+    return int(_lib.load().uwir_cross_attn_workspace_bytes(B, nq, nk, heads, kv_heads, hd, _torch_dt(dtype)))
+
+
+def cross_attn_backward_workspace_bytes(B: int, nq: int, nk: int, heads: int, kv_heads: int, hd: int, dtype: torch.dtype) -> int:
+    return int(_lib.load().uwir_cross_attn_backward_workspace_bytes(B, nq, nk, heads, kv_heads, hd, _torch_dt(dtype)))
+
+
+def _xattn_check(what, q, B, nq, nk, heads, kv_heads, hd, rows, keys, key_lens, key_mask, lse, workspace):
+    if B < 1 or nq < 0 or nk < 0 or heads < 1 or kv_heads < 1 or heads % kv_heads or hd < 1:
+        raise ValueError(f"{what}: need B > 0, nq, nk >= 0 and kv_heads dividing heads")
+    for name, t in rows:
+        _rows_cols(what, name, t, B * nq, heads * hd)
+    for name, t in keys:
+        _rows_cols(what, name, t, B * nk, kv_heads * hd)
+    if any(t.dtype != q.dtype for _, t in rows + keys):
+        raise TypeError(f"{what}: {', '.join(n for n, _ in rows + keys)} must share a dtype")
+    if key_lens is not None and (key_lens.dtype != torch.int32 or tuple(key_lens.shape) != (B,) or not key_lens.is_contiguous()):
+        raise ValueError(f"{what}: key_lens must be a contiguous int32 [{B}]")
+    if key_mask is not None:
+        if key_mask.dtype not in (torch.bool, torch.uint8):
+            raise TypeError(f"{what}: key_mask must be bool or uint8")
+        _rows_cols(what, "key_mask", key_mask, B, nk)
+    _vector(what, "lse", lse, B, heads, nq)
+    if workspace is not None and not workspace.is_contiguous():
+        raise ValueError(f"{what}: workspace must be contiguous")
+    _operands(what, q, *(t for _, t in rows + keys), key_lens, key_mask, lse, workspace)
+
+
+def cross_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, B: int, nq: int, nk: int, heads: int, kv_heads: int, hd: int,
+               scale: float, out: torch.Tensor, workspace: Optional[torch.Tensor] = None, key_lens: Optional[torch.Tensor] = None,
+               key_mask: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None) -> None:
+    """out = softmax(scale q k^T) v over the visible keys of each image; q, out [B * nq, heads * hd], k, v [B * nk, kv_heads * hd]
+    (fp32 or bf16, one dtype), head h reads key head h // (heads // kv_heads).  Visible: index < key_lens[b] (int32 [B]) and
+    key_mask[b, index] (bool [B, nk]).  ``lse`` [B, heads, nq] fp32 keeps log sum exp for ``cross_attn_backward``.  An image
+    without visible keys gives zeros (lse = -inf).  workspace: cross_attn_workspace_bytes (None if that is 0); see uwir.h."""
+    what = "cross_attn"
+    _xattn_check(what, q, B, nq, nk, heads, kv_heads, hd, [("q", q), ("out", out)], [("k", k), ("v", v)], key_lens, key_mask, lse,
+                 workspace)
+    _lib.check(_lib.load().uwir_cross_attn(
+        _p(q), _row_stride(q), _p(k), _row_stride(k), _p(v), _row_stride(v), _dt(q), B, nq, nk, heads, kv_heads, hd, scale,
+        _p(key_lens), _p(key_mask), 0 if key_mask is None else _row_stride(key_mask), _p(out), _row_stride(out), _p(lse),
+        _p(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(), _stream(q)), what)
+
+
+def cross_attn_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, lse: torch.Tensor, dout: torch.Tensor,
+                        B: int, nq: int, nk: int, heads: int, kv_heads: int, hd: int, scale: float, dq: torch.Tensor,
+                        dk: torch.Tensor, dv: torch.Tensor, workspace: torch.Tensor, key_lens: Optional[torch.Tensor] = None,
+                        key_mask: Optional[torch.Tensor] = None) -> None:
+    """Gradients of ``cross_attn`` from its out and lse: dq like q, dk / dv like k / v (written, not added to; zeros at
+    invisible keys; summed over the query heads of a shared key head)."""
+    what = "cross_attn_backward"
+    _xattn_check(what, q, B, nq, nk, heads, kv_heads, hd, [("q", q), ("out", out), ("dout", dout), ("dq", dq)],
+                 [("k", k), ("v", v), ("dk", dk), ("dv", dv)], key_lens, key_mask, lse, workspace)
+    _lib.check(_lib.load().uwir_cross_attn_backward(
+        _p(q), _row_stride(q), _p(k), _row_stride(k), _p(v), _row_stride(v), _p(out), _row_stride(out), _p(lse), _p(dout),
+        _row_stride(dout), _dt(q), B, nq, nk, heads, kv_heads, hd, scale, _p(key_lens), _p(key_mask),
+        0 if key_mask is None else _row_stride(key_mask), _p(dq), _row_stride(dq), _p(dk), _row_stride(dk), _p(dv),
+        _row_stride(dv), _p(workspace), workspace.numel() * workspace.element_size(), _stream(q)), what)
+
+
 def fft_workspace_bytes(B: int, H: int, W: int, C_: int) -> int:
     return int(_lib.load().uwir_fft_workspace_bytes(B, H, W, C_))
 
@@ -633,6 +786,7 @@ def _census_wrap(name: str, fn):
 for _n in ("dwt2", "idwt2", "ln2d_affine", "conv_gemm", "dwconv_ms", "flash_attn", "fft2_amp_phase", "ifft2_polar_add",
            "affine_cast", "stem_conv3x3", "head_conv3x3", "sde_euler_step", "sde_posterior_step", "linear_attention",
            "ln_rows", "groupnorm_affine", "geglu", "linattn_block", "tail_conv3x3", "unet_input", "bilinear_nchw_to_nhwc", "linear",
-           "gate_idwt", "gate_blend", "ffn_fused", "fold_affine_weights"):
+           "gate_idwt", "gate_blend", "ffn_fused", "fold_affine_weights", "group_norm_act", "group_norm_act_backward", "cross_attn",
+           "cross_attn_backward"):
     globals()[_n] = _census_wrap(_n, globals()[_n])
 del _n
