@@ -16,10 +16,12 @@ SOURCES = ["elementwise.hip", "dwconv.hip", "gemm.hip", "gemm_wide.hip", "gemm_w
            "teacher.hip", "enhance.hip", "enhance_cv.hip", "groupnorm.hip", "cross_attn.hip",
            "cross_attn_bwd.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+# -packed-fp32-ops: no packed fp32 arithmetic, some forms of which give wrong results on this part (the host pass of hipcc
+# says that it does not know the feature: harmless).
 # -amdgpu-mfma-vgpr-form: keep MFMA accumulators in VGPRs (gfx950 has a unified file); without it every softmax /
 # epilogue touch of an accumulator costs a v_accvgpr_read/write pair.
 FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function",
-         "-mllvm", "-amdgpu-mfma-vgpr-form=1"]
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-mllvm", "-amdgpu-mfma-vgpr-form=1"]
 
 
 def _stale(target: str, deps) -> bool:
