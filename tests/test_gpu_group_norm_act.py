@@ -91,7 +91,8 @@ def close(got, want, tol, half):
 
 # n = 1, one element a group (variance 0), odd channel counts, unaligned groups, both forms, one group over everything
 SHAPES = [(1, 1, 8, 8), (2, 1, 32, 4), (1, 64, 512, 32), (3, 418, 96, 32), (2, 33, 15, 5), (2, 1500, 30, 3), (1, 5000, 64, 32),
-          (2, 700, 1024, 1), (5, 17, 2048, 32), (1, 2049, 2048, 2048), (2, 4100, 396, 4), (16, 1024, 128, 32), (1, 70001, 6, 2)]
+          (2, 700, 1024, 1), (5, 17, 2048, 32), (1, 2049, 2048, 2048), (2, 4100, 396, 4), (16, 1024, 128, 32), (1, 70001, 6, 2),
+          (2, 900, 1026, 2), (2, 900, 1026, 1), (1, 700, 2047, 1), (3, 5000, 192, 64), (1, 3000, 160, 4)]
 
 
 @pytest.mark.parametrize("dt,do", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.float32, torch.bfloat16),

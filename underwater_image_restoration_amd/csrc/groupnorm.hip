@@ -1,11 +1,12 @@
 // Group norm with an activation on NHWC rows, forward and backward.
 //   mean, var over the n x cg elements of (image, group);  xh = (x - mean) rstd
 //   z = (xh gamma + beta)(1 + scale_b) + shift_b;   y = act(z),  act = identity or SiLU
-// Both directions are bound by memory (or, for small maps, by launch latency).  Two forms:
-//   resident  a block owns a slab of whole groups of one image, keeps its rows in registers between the statistics and
-//             the output, and so touches every element once (one launch);
-//   streamed  statistics of row chunks in one launch, output in the next; the second read of x comes from the L2 / the
-//             memory-side cache where the map fits.
+// Both directions are bound by memory (or, for small maps, by launch latency).  A block owns a slab of whole groups (at
+// least 64 bytes of a row, 128 where the map is streamed: full cache lines) and some rows of one image:
+//   resident  all rows: they stay in registers between the statistics and the output, every element is touched once and
+//             there is one launch
+//   streamed  a chunk of rows: statistics in one launch, output in the next; the second read of x comes from the L2 (the
+//             same block index runs on the same XCD) or the memory-side cache where the map fits
 // Statistics: every thread reduces batches of rows to (mean, sum of squared distances to that mean) per channel and
 // merges them pairwise, so that a mean far from zero or a stray first element costs no digits; everything across
 // threads is summed in fp64 in a fixed order (results do not depend on scheduling).
@@ -14,10 +15,10 @@
 
 namespace {
 
-constexpr int GN_T = 256;          // threads of the streaming kernels
+constexpr int GN_T = 512;          // threads of the streaming kernels
 constexpr int GN_R = 8;            // rows a thread loads ahead of using them
-constexpr int GN_MAX_C = 2048;     // per-channel fp64 sums of one block live in LDS
-constexpr int GN_MAX_CHUNKS = 128; // row chunks of an image (each output block sums all of an image's partials)
+constexpr int GN_MAX_C = 2048;     // channels of a group, and so of a slab, are bounded by the per-slab sums in LDS
+constexpr int GN_MAX_CHUNKS = 128; // row chunks of an image (each output block sums all partials of its slab)
 
 template <typename T, int V> struct VecT { typedef T type __attribute__((ext_vector_type(V))); };
 template <typename T> struct VecT<T, 1> { typedef T type; };
@@ -43,11 +44,13 @@ struct GnArgs {
     const float *mean_in, *rstd_in;  // backward
     float *mean, *rstd;              // forward, optional
     float *dgamma, *dbeta, *dss;     // backward; dss [B, ld_dss] optional
-    double2* part;                   // forward partials [B][chunks][G]: (sum, sum of squares)
+    double2* part;                   // forward partials [B][G][chunks]: (sum, sum of squares)
     float2* cpart;                   // backward partials [B][chunks][C]: (sum dz, sum dz xh)
-    float2* csum;                    // backward [B][C]
+    float2* csum;                    // the same summed over the chunks, [B][C]
+    const float2* sums;              // what the output pass reads: cpart or csum, [B][sum_chunks][C]
     size_t ldx, ldy, ldo, ld_ss, ld_dss;
-    int B, n, C, G, cg, chunks, rows, slab;  // rows per chunk; channels per slab
+    double inv_n;                    // 1 / (n cg)
+    int B, n, C, G, cg, chunks, rows, slab, sum_chunks;  // rows per chunk; channels per slab
     float eps;
     int act;
 };
@@ -62,20 +65,19 @@ template <int V> struct Stat {
         for (int j = 0; j < V; ++j) mean[j] = m2[j] = 0.f;
     }
     // merge `k` <= GN_R fresh rows (pairwise update: exact in the count weights)
-    template <typename T> __device__ __forceinline__ void batch(const Pack<T, V>* p, int k) {
-        if (k <= 0) return;
-        const float inv = 1.f / (float)k;
+    template <bool FULL, typename T> __device__ __forceinline__ void merge(const Pack<T, V>* p, int k) {
+        const float inv = FULL ? 1.f / GN_R : 1.f / (float)k;
         const float wa = (float)k / (float)(cnt + k), wb = (float)cnt * wa;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             float s = 0.f;
 #pragma unroll
-            for (int i = 0; i < GN_R; ++i) s += i < k ? p[i].get(j) : 0.f;
+            for (int i = 0; i < GN_R; ++i) s += FULL || i < k ? p[i].get(j) : 0.f;
             const float m = s * inv;
             float q = 0.f;
 #pragma unroll
             for (int i = 0; i < GN_R; ++i) {
-                const float d = i < k ? p[i].get(j) - m : 0.f;
+                const float d = FULL || i < k ? p[i].get(j) - m : 0.f;
                 q = fmaf(d, d, q);
             }
             const float d = m - mean[j];
@@ -84,38 +86,77 @@ template <int V> struct Stat {
         }
         cnt += k;
     }
+    template <typename T> __device__ __forceinline__ void batch(const Pack<T, V>* p, int k) {
+        if (k == GN_R) merge<true>(p, k);
+        else if (k > 0) merge<false>(p, k);
+    }
 };
+
+// rows r, r + step, ... (k <= R of them; the others repeat row r, which must exist)
+template <int R, typename T, int V>
+__device__ __forceinline__ void load_rows(Pack<T, V>* buf, const T* src, size_t ld, int r, int step, int k) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) buf[i].load(src + (size_t)(i < k ? r + i * step : r) * ld);
+}
+
+// walks a thread's rows r, r + step, ... < r1: f(r, R) for full batches of R rows (k is then a constant), f(r, k) for the rest
+template <int R, typename F> __device__ __forceinline__ void row_batches(int r, int r1, int step, F f) {
+    for (; r + (R - 1) * step < r1; r += R * step) f(r, R);
+    if (r < r1) f(r, (r1 - r + step - 1) / step);
+}
 
 __device__ __forceinline__ double shfl_xor_d(double v, int m) {
     return __hiloint2double(__shfl_xor(__double2hiint(v), m), __shfl_xor(__double2loint(v), m));
 }
 
-// threads that share one group's reduction: a power of two <= 64 with tpg * G <= T where that is possible
-__device__ __forceinline__ int threads_per_group(int G, int T) {
-    int t = 64;
-    while (t > 1 && t * G > T) t >>= 1;
-    return t;
-}
-
-// sums over groups of f(g, i) for i in [0, m): result in every lane of the group's team, handed to `done(g, a, b)` by lane 0
-template <typename F, typename D>
-__device__ __forceinline__ void group_sums(int G, int m, int tid, int T, F f, D done) {
-    const int tpg = threads_per_group(G, T), teams = T / tpg, lane = tid & (tpg - 1);
-    for (int g0 = 0; g0 < G; g0 += teams) {   // uniform trip count: the shuffles below see whole waves
-        const int g = g0 + tid / tpg;
+// Sums of f(g, i), i in [0, m), for every group g of a block, handed to done(g, sum) by one thread each.  Teams of up to a
+// wave; with fewer groups than teams several teams share a group and `scratch` [T / 64 at most] joins them.  Ends with a barrier.
+template <int T, typename F, typename D>
+__device__ __forceinline__ void group_sums(int G, int m, int tid, double2* scratch, F f, D done) {
+    int tpg = 64;
+    while (tpg > 1 && tpg * G > T) tpg >>= 1;
+    const int teams = T / tpg, lane = tid & (tpg - 1), team = tid / tpg;
+    if (G * 2 <= teams) {   // only with whole-wave teams
+        const int parts = teams / G, g = team % G, part = team / G;
         double a = 0., b = 0.;
-        if (g < G)
-            for (int i = lane; i < m; i += tpg) {
+        if (part < parts)
+            for (int i = part * 64 + lane; i < m; i += parts * 64) {
                 const double2 v = f(g, i);
                 a += v.x;
                 b += v.y;
             }
-        for (int o = tpg >> 1; o; o >>= 1) {
+        for (int o = 32; o; o >>= 1) {
             a += shfl_xor_d(a, o);
             b += shfl_xor_d(b, o);
         }
-        if (g < G && lane == 0) done(g, a, b);
+        if (lane == 0) scratch[team] = make_double2(a, b);
+        __syncthreads();
+        if (tid < G) {
+            a = b = 0.;
+            for (int q = 0; q < parts; ++q) {
+                a += scratch[q * G + tid].x;
+                b += scratch[q * G + tid].y;
+            }
+            done(tid, a, b);
+        }
+    } else {
+        for (int g0 = 0; g0 < G; g0 += teams) {   // uniform trip count: the shuffles see whole waves
+            const int g = g0 + team;
+            double a = 0., b = 0.;
+            if (g < G)
+                for (int i = lane; i < m; i += tpg) {
+                    const double2 v = f(g, i);
+                    a += v.x;
+                    b += v.y;
+                }
+            for (int o = tpg >> 1; o; o >>= 1) {
+                a += shfl_xor_d(a, o);
+                b += shfl_xor_d(b, o);
+            }
+            if (g < G && lane == 0) done(g, a, b);
+        }
     }
+    __syncthreads();
 }
 
 __device__ __forceinline__ float act_silu(float z) { return z * sigmoid_fast(z); }
@@ -124,30 +165,118 @@ __device__ __forceinline__ float dact_silu(float z) {
     return s * fmaf(z, 1.f - s, 1.f);
 }
 
+// where a block's thread works: its slab of one image, a vector of V channels, row lane rl of RL
+struct Place {
+    int b, ch0, sc, tw, RL, cv, rl;
+    template <int V> __device__ __forceinline__ static Place of(const GnArgs& p, int slab, int b, int tid, int T) {
+        Place l;
+        l.b = b;
+        l.ch0 = slab * p.slab;
+        l.sc = min(p.slab, p.C - l.ch0);
+        l.tw = l.sc / V;
+        l.RL = l.tw <= T ? T / l.tw : 1;
+        l.cv = tid % l.tw;
+        l.rl = tid / l.tw;
+        return l;
+    }
+};
+
+// sums of the block's rows per group from the threads' statistics in LDS; `total` rows were dealt to RL row lanes in turn
+template <int T, int V, typename D>
+__device__ __forceinline__ void slab_group_sums(const GnArgs& p, const Place& l, int width, int groups, int total, const float* sm,
+                                                const float* sq, double2* scratch, int tid, D done) {
+    const int cg = p.cg, rows = min(l.RL, max(total, 0)), base = total > 0 ? total / l.RL : 0, rem = total > 0 ? total % l.RL : 0;
+    group_sums<T>(groups, cg * rows, tid, scratch,
+                  [&](int g, int i) {
+                      const int r = i / cg, c = i - r * cg, at = r * width + g * cg + c;
+                      const double k = base + (r < rem), m = sm[at];
+                      return make_double2(k * m, (double)sq[at] + k * m * m);
+                  },
+                  done);
+}
+
+__device__ __forceinline__ float2 finish_stats(double s, double q, double inv_n, float eps) {
+    const double m = s * inv_n;
+    const float v = (float)fmax(q * inv_n - m * m, 0.);
+    return make_float2((float)m, rsqrtf(v + eps));
+}
+
+// per-channel coefficients of a thread's V channels: z = (x - m) a + s, xh = (x - m) r; gamma, beta and the modulation are
+// loaded ahead of the statistics
+template <int V> struct Coef {
+    float w[V], s[V], m[V], r[V];   // w = gamma (1 + scale)
+    __device__ __forceinline__ void load(const GnArgs& p, int b, int c0) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int c = c0 + j;
+            w[j] = p.gamma[c];
+            s[j] = p.beta[c];
+            if (p.ss) {
+                const float f = 1.f + p.ss[(size_t)b * p.ld_ss + c];
+                w[j] *= f;
+                s[j] = fmaf(s[j], f, p.ss[(size_t)b * p.ld_ss + p.C + c]);
+            }
+        }
+    }
+    __device__ __forceinline__ void stats(int j, float mean, float rstd) {
+        m[j] = mean;
+        r[j] = rstd;
+        w[j] *= rstd;               // now a
+    }
+    __device__ __forceinline__ float z(int j, float d) const { return fmaf(d, w[j], s[j]); }
+};
+
+template <int R, typename TX, typename TO, int V>
+__device__ __forceinline__ void emit(const Pack<TX, V>* buf, const Coef<V>& co, TO* dst, size_t ld, int r, int step, int k, bool silu) {
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+        if (i < k) {
+            Pack<TO, V> o;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float z = co.z(j, buf[i].get(j) - co.m[j]);
+                o.set(j, silu ? act_silu(z) : z);
+            }
+            o.store(dst + (size_t)(r + i * step) * ld);
+        }
+}
+
 // ---------------------------------------------------------------------------------------- forward, streamed
+// A slab wider than the block (one group over more than GN_T vectors) is walked in tiles of GN_T vectors; the groups are then
+// summed tile by tile through `ch`.
 template <typename TX, int V>
 __global__ void __launch_bounds__(GN_T) gn_stats_kernel(GnArgs p) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    float* sm = reinterpret_cast<float*>(smem);                        // [GN_T][V] means
+    double2* scratch = reinterpret_cast<double2*>(smem);               // [GN_T / 64]
+    float* sm = reinterpret_cast<float*>(scratch + GN_T / 64);         // [GN_T][V] means
     float* sq = sm + GN_T * V;                                         // [GN_T][V] squares
-    double2* ch = reinterpret_cast<double2*>(sq + GN_T * V);           // [C] (sum, sum of squares)
-    const int tid = threadIdx.x, chunk = blockIdx.x, b = blockIdx.y;
-    const int nv = p.C / V;
+    const int tid = threadIdx.x, chunk = blockIdx.x, b = blockIdx.z;
+    const Place l = Place::of<V>(p, blockIdx.y, b, tid, GN_T);
     const int r0 = chunk * p.rows, r1 = min(p.n, r0 + p.rows);
-    const TX* X = (const TX*)p.x + (size_t)b * p.n * p.ldx;
-    for (int c0 = 0; c0 < nv; c0 += GN_T) {
-        const int tw = min(nv - c0, GN_T), RL = GN_T / tw, cv = tid % tw, rl = tid / tw;
+    const TX* X = (const TX*)p.x + (size_t)b * p.n * p.ldx + l.ch0;
+    double2* out = p.part + ((size_t)b * p.G + l.ch0 / p.cg) * p.chunks + chunk;
+    double wide_s = 0., wide_q = 0.;
+    for (int v0 = 0; v0 < l.tw; v0 += GN_T) {
+        const bool wide = l.tw > GN_T;
+        const int cv = wide ? v0 + tid : l.cv;
         Stat<V> st;
         st.clear();
-        if (rl < RL) {
-            const TX* src = X + (size_t)(c0 + cv) * V;
-            for (int r = r0 + rl; r < r1; r += RL * GN_R) {
+        if (wide ? cv < l.tw : l.rl < l.RL) {
+            const TX* src = X + (size_t)cv * V;
+            row_batches<GN_R>(r0 + (wide ? 0 : l.rl), r1, l.RL, [&](int r, int k) {
                 Pack<TX, V> buf[GN_R];
-                const int k = min(GN_R, (r1 - r + RL - 1) / RL);
-#pragma unroll
-                for (int i = 0; i < GN_R; ++i) buf[i].load(src + (size_t)(i < k ? r + i * RL : r) * p.ldx);
+                load_rows<GN_R>(buf, src, p.ldx, r, l.RL, k);
                 st.batch(buf, k);
+            });
+        }
+        if (wide) {   // a single group: the thread's own sums
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const double k = st.cnt, m = st.mean[j];
+                wide_s += k * m;
+                wide_q += (double)st.m2[j] + k * m * m;
             }
+            continue;
         }
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -155,95 +284,61 @@ __global__ void __launch_bounds__(GN_T) gn_stats_kernel(GnArgs p) {
             sq[tid * V + j] = st.m2[j];
         }
         __syncthreads();
-        for (int c = tid; c < tw * V; c += GN_T) {
-            double s = 0., q = 0.;
-            for (int l = 0; l < RL; ++l) {
-                const int left = r1 - r0 - l;
-                const double k = left > 0 ? (left + RL - 1) / RL : 0;
-                const double m = sm[l * tw * V + c];
-                s += k * m;
-                q += sq[l * tw * V + c] + k * m * m;
-            }
-            ch[c0 * V + c] = make_double2(s, q);
-        }
+        slab_group_sums<GN_T, V>(p, l, l.sc, l.sc / p.cg, r1 - r0, sm, sq, scratch, tid,
+                                 [&](int g, double s, double q) { out[(size_t)g * p.chunks] = make_double2(s, q); });
+    }
+    if (l.tw > GN_T) {
+        double2* all = scratch + GN_T / 64;   // [GN_T], in the place of sm and sq
+        all[tid] = make_double2(wide_s, wide_q);
         __syncthreads();
+        group_sums<GN_T>(1, GN_T, tid, scratch, [&](int, int i) { return all[i]; },
+                         [&](int, double s, double q) { out[0] = make_double2(s, q); });
     }
-    double2* out = p.part + ((size_t)b * p.chunks + chunk) * p.G;
-    const int cg = p.cg;
-    group_sums(p.G, cg, tid, GN_T, [&](int g, int i) { return ch[g * cg + i]; },
-               [&](int g, double s, double q) { out[g] = make_double2(s, q); });
-}
-
-__device__ __forceinline__ float2 finish_stats(double s, double q, double N, float eps) {
-    const double m = s / N;
-    double v = q / N - m * m;
-    v = v > 0. ? v : 0.;
-    return make_float2((float)m, (float)(1. / sqrt(v + (double)eps)));
-}
-
-// folded per-channel coefficients: z = (x - m) a + s
-__device__ __forceinline__ void channel_affine(const GnArgs& p, int b, int c, float rstd, float& a, float& s) {
-    const float ga = p.gamma[c], be = p.beta[c];
-    float f = 1.f, sh = 0.f;
-    if (p.ss) {
-        f = 1.f + p.ss[(size_t)b * p.ld_ss + c];
-        sh = p.ss[(size_t)b * p.ld_ss + p.C + c];
-    }
-    a = rstd * ga * f;
-    s = fmaf(be, f, sh);
 }
 
 template <typename TX, typename TO, int V>
-__global__ void __launch_bounds__(GN_T) gn_apply_kernel(GnArgs p) {
+__global__ void __launch_bounds__(GN_T, 4) gn_apply_kernel(GnArgs p) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    float2* gst = reinterpret_cast<float2*>(smem);   // [G] (mean, rstd)
-    const int tid = threadIdx.x, chunk = blockIdx.x, b = blockIdx.y;
-    const int nv = p.C / V, cg = p.cg;
-    const double2* part = p.part + (size_t)b * p.chunks * p.G;
-    const double N = (double)p.n * cg;
-    group_sums(p.G, p.chunks, tid, GN_T, [&](int g, int i) { return part[(size_t)i * p.G + g]; },
-               [&](int g, double s, double q) {
-                   const float2 st = finish_stats(s, q, N, p.eps);
-                   gst[g] = st;
-                   if (chunk == 0) {
-                       if (p.mean) p.mean[(size_t)b * p.G + g] = st.x;
-                       if (p.rstd) p.rstd[(size_t)b * p.G + g] = st.y;
-                   }
-               });
-    __syncthreads();
+    double2* scratch = reinterpret_cast<double2*>(smem);               // [GN_T / 64]
+    float2* gst = reinterpret_cast<float2*>(scratch + GN_T / 64);      // [slab / cg] (mean, rstd)
+    const int tid = threadIdx.x, chunk = blockIdx.x, b = blockIdx.z;
+    const Place l = Place::of<V>(p, blockIdx.y, b, tid, GN_T);
+    const int cg = p.cg, g0 = l.ch0 / cg;
     const int r0 = chunk * p.rows, r1 = min(p.n, r0 + p.rows);
-    const TX* X = (const TX*)p.x + (size_t)b * p.n * p.ldx;
-    TO* Y = (TO*)p.out + (size_t)b * p.n * p.ldo;
-    const bool silu = p.act == UWIR_ACT_SILU;
-    for (int c0 = 0; c0 < nv; c0 += GN_T) {
-        const int tw = min(nv - c0, GN_T), RL = GN_T / tw, cv = tid % tw, rl = tid / tw;
-        if (rl >= RL) continue;
-        const int cb = (c0 + cv) * V;
-        float m[V], a[V], s[V];
+    const TX* X = (const TX*)p.x + (size_t)b * p.n * p.ldx + l.ch0;
+    TO* Y = (TO*)p.out + (size_t)b * p.n * p.ldo + l.ch0;
+    const bool silu = p.act == UWIR_ACT_SILU, wide = l.tw > GN_T;
+    Coef<V> co;
+    const bool works = !wide && l.rl < l.RL && r0 + l.rl < r1;
+    if (works) co.load(p, b, l.ch0 + l.cv * V);   // on their way while the statistics are put together
+    const double2* part = p.part + ((size_t)b * p.G + g0) * p.chunks;
+    group_sums<GN_T>(l.sc / cg, p.chunks, tid, scratch, [&](int g, int i) { return part[(size_t)g * p.chunks + i]; },
+                     [&](int g, double s, double q) {
+                         const float2 st = finish_stats(s, q, p.inv_n, p.eps);
+                         gst[g] = st;
+                         if (chunk == 0) {
+                             if (p.mean) p.mean[(size_t)b * p.G + g0 + g] = st.x;
+                             if (p.rstd) p.rstd[(size_t)b * p.G + g0 + g] = st.y;
+                         }
+                     });
+    auto walk = [&](int cv, int r, int step) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const float2 st = gst[(cb + j) / cg];
-            m[j] = st.x;
-            channel_affine(p, b, cb + j, st.y, a[j], s[j]);
+            const float2 st = gst[wide ? 0 : (cv * V + j) / cg];
+            co.stats(j, st.x, st.y);
         }
-        for (int r = r0 + rl; r < r1; r += RL * GN_R) {
-            Pack<TX, V> buf[GN_R];
-            const int k = min(GN_R, (r1 - r + RL - 1) / RL);
-#pragma unroll
-            for (int i = 0; i < GN_R; ++i) buf[i].load(X + (size_t)(i < k ? r + i * RL : r) * p.ldx + cb);
-#pragma unroll
-            for (int i = 0; i < GN_R; ++i)
-                if (i < k) {
-                    Pack<TO, V> o;
-#pragma unroll
-                    for (int j = 0; j < V; ++j) {
-                        const float z = fmaf(buf[i].get(j) - m[j], a[j], s[j]);
-                        o.set(j, silu ? act_silu(z) : z);
-                    }
-                    o.store(Y + (size_t)(r + i * RL) * p.ldo + cb);
-                }
+        row_batches<GN_R / 2>(r, r1, step, [&](int r, int k) {
+            Pack<TX, V> buf[GN_R / 2];
+            load_rows<GN_R / 2>(buf, X + cv * V, p.ldx, r, step, k);
+            emit<GN_R / 2>(buf, co, Y + cv * V, p.ldo, r, step, k, silu);
+        });
+    };
+    if (works) walk(l.cv, r0 + l.rl, l.RL);
+    if (wide)
+        for (int cv = tid; cv < l.tw; cv += GN_T) {
+            co.load(p, b, l.ch0 + cv * V);
+            walk(cv, r0, 1);
         }
-    }
 }
 
 // ---------------------------------------------------------------------------------------- forward, resident
@@ -252,17 +347,18 @@ __global__ void __launch_bounds__(T) gn_resident_kernel(GnArgs p) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     float* sm = reinterpret_cast<float*>(smem);
     float* sq = sm + T * V;
-    double2* ch = reinterpret_cast<double2*>(sq + T * V);              // [slab]
-    float2* gst = reinterpret_cast<float2*>(ch + p.slab);              // [slab / cg]
+    double2* scratch = reinterpret_cast<double2*>(sq + T * V);         // [T / 64]
+    float2* gst = reinterpret_cast<float2*>(scratch + T / 64);         // [slab / cg]
     const int tid = threadIdx.x, b = blockIdx.y, cg = p.cg;
-    const int ch0 = blockIdx.x * p.slab, sc = min(p.slab, p.C - ch0), gs = sc / cg, g0 = ch0 / cg;
-    const int tw = sc / V, RL = T / tw, cv = tid % tw, rl = tid / tw;
-    const TX* X = (const TX*)p.x + (size_t)b * p.n * p.ldx + ch0 + cv * V;
+    const Place l = Place::of<V>(p, blockIdx.x, b, tid, T);
+    const int g0 = l.ch0 / cg;
+    const TX* X = (const TX*)p.x + (size_t)b * p.n * p.ldx + l.ch0 + l.cv * V;
     Pack<TX, V> buf[GN_R];
-    const int k = rl < RL && rl < p.n ? (p.n - rl + RL - 1) / RL : 0;  // <= GN_R by the launch rule
+    Coef<V> co;
+    const int k = l.rl < l.RL && l.rl < p.n ? (p.n - l.rl + l.RL - 1) / l.RL : 0;  // <= GN_R by the launch rule
     if (k > 0) {
-#pragma unroll
-        for (int i = 0; i < GN_R; ++i) buf[i].load(X + (size_t)(i < k ? rl + i * RL : rl) * p.ldx);
+        load_rows<GN_R>(buf, X, p.ldx, l.rl, l.RL, k);
+        co.load(p, b, l.ch0 + l.cv * V);
     }
     Stat<V> st;
     st.clear();
@@ -273,138 +369,143 @@ __global__ void __launch_bounds__(T) gn_resident_kernel(GnArgs p) {
         sq[tid * V + j] = st.m2[j];
     }
     __syncthreads();
-    const int rows = min(RL, p.n);
-    for (int c = tid; c < sc; c += T) {
-        double s = 0., q = 0.;
-        for (int l = 0; l < rows; ++l) {
-            const double kk = (p.n - l + RL - 1) / RL, m = sm[l * sc + c];
-            s += kk * m;
-            q += sq[l * sc + c] + kk * m * m;
-        }
-        ch[c] = make_double2(s, q);
-    }
-    __syncthreads();
-    const double N = (double)p.n * cg;
-    group_sums(gs, cg, tid, T, [&](int g, int i) { return ch[g * cg + i]; },
-               [&](int g, double s, double q) {
-                   const float2 f = finish_stats(s, q, N, p.eps);
-                   gst[g] = f;
-                   if (p.mean) p.mean[(size_t)b * p.G + g0 + g] = f.x;
-                   if (p.rstd) p.rstd[(size_t)b * p.G + g0 + g] = f.y;
-               });
-    __syncthreads();
+    slab_group_sums<T, V>(p, l, l.sc, l.sc / cg, p.n, sm, sq, scratch, tid, [&](int g, double s, double q) {
+        const float2 f = finish_stats(s, q, p.inv_n, p.eps);
+        gst[g] = f;
+        if (p.mean) p.mean[(size_t)b * p.G + g0 + g] = f.x;
+        if (p.rstd) p.rstd[(size_t)b * p.G + g0 + g] = f.y;
+    });
     if (k <= 0) return;
-    const bool silu = p.act == UWIR_ACT_SILU;
-    float m[V], a[V], s[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const float2 f = gst[(cv * V + j) / cg];
-        m[j] = f.x;
-        channel_affine(p, b, ch0 + cv * V + j, f.y, a[j], s[j]);
+        const float2 f = gst[(l.cv * V + j) / cg];
+        co.stats(j, f.x, f.y);
     }
-    TO* Y = (TO*)p.out + (size_t)b * p.n * p.ldo + ch0 + cv * V;
+    emit<GN_R>(buf, co, (TO*)p.out + (size_t)b * p.n * p.ldo + l.ch0 + l.cv * V, p.ldo, l.rl, l.RL, k, p.act == UWIR_ACT_SILU);
+}
+
+// ---------------------------------------------------------------------------------------- backward
+// SiLU's derivative costs an exponential and a reciprocal per element (8 of about 20 issue slots): it, not memory, bounds the
+// bf16 passes.  With d = x - m the sums need dz and dz d only (xh = d r enters once per channel).
+template <int V, typename T>
+__device__ __forceinline__ void bwd_stats(const GnArgs& p, Coef<V>& co, int b, int c0) {
+    co.load(p, b, c0);
 #pragma unroll
-    for (int i = 0; i < GN_R; ++i)
+    for (int j = 0; j < V; ++j) {
+        const int g = (c0 + j) / p.cg;
+        co.stats(j, p.mean_in[(size_t)b * p.G + g], p.rstd_in[(size_t)b * p.G + g]);
+    }
+}
+
+// adds a batch of rows: s1 += sum dz, s2 += sum dz d.  A short chain per batch keeps the fp32 sums close to pairwise.
+template <int R, typename T, int V>
+__device__ __forceinline__ void bwd_batch(const Pack<T, V>* bx, const Pack<T, V>* bd, const Coef<V>& co, int k, bool silu, float* s1,
+                                          float* s2) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        float t1 = 0.f, t2 = 0.f;
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+            if (i < k) {
+                const float d = bx[i].get(j) - co.m[j];
+                float dz = bd[i].get(j);
+                if (silu) dz *= dact_silu(co.z(j, d));
+                t1 += dz;
+                t2 = fmaf(dz, d, t2);
+            }
+        s1[j] += t1;
+        s2[j] += t2;
+    }
+}
+
+// dx = r (w dz - m1 - xh m2) with u1 = r m1, u2 = r^2 m2
+template <int R, typename T, int V>
+__device__ __forceinline__ void bwd_emit(const Pack<T, V>* bx, const Pack<T, V>* bd, const Coef<V>& co, const float* u1, const float* u2,
+                                         T* dst, size_t ld, int r, int step, int k, bool silu) {
+#pragma unroll
+    for (int i = 0; i < R; ++i)
         if (i < k) {
-            Pack<TO, V> o;
+            Pack<T, V> o;
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float z = fmaf(buf[i].get(j) - m[j], a[j], s[j]);
-                o.set(j, silu ? act_silu(z) : z);
+                const float d = bx[i].get(j) - co.m[j];
+                float dz = bd[i].get(j);
+                if (silu) dz *= dact_silu(co.z(j, d));
+                o.set(j, fmaf(co.w[j], dz, -fmaf(d, u2[j], u1[j])));
             }
-            o.store(Y + (size_t)(rl + i * RL) * p.ldo);
+            o.store(dst + (size_t)(r + i * step) * ld);
         }
 }
 
-// ---------------------------------------------------------------------------------------- backward, streamed
-// per-channel coefficients of a thread: z = (x - m) a + s, xh = (x - m) r
-template <int V> struct BwdCoef {
-    float m[V], r[V], a[V], s[V];
-    __device__ __forceinline__ void load(const GnArgs& p, int b, int c0) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int c = c0 + j, g = c / p.cg;
-            m[j] = p.mean_in[(size_t)b * p.G + g];
-            r[j] = p.rstd_in[(size_t)b * p.G + g];
-            channel_affine(p, b, c, r[j], a[j], s[j]);
-        }
-    }
-    __device__ __forceinline__ void grad(int j, float x, float dy, bool silu, float& dz, float& xh) const {
-        const float d = x - m[j];
-        xh = d * r[j];
-        dz = silu ? dy * dact_silu(fmaf(d, a[j], s[j])) : dy;
-    }
-};
+constexpr int GN_RB = 2;   // rows a thread has in flight, x and dy each: coefficients fill the registers, waves hide the latency
 
 template <typename T, int V>
-__global__ void __launch_bounds__(GN_T) gn_bwd_sums_kernel(GnArgs p) {
+__global__ void __launch_bounds__(GN_T, 4) gn_bwd_sums_kernel(GnArgs p) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     float2* red = reinterpret_cast<float2*>(smem);   // [GN_T][V]
-    const int tid = threadIdx.x, chunk = blockIdx.x, b = blockIdx.y;
-    const int nv = p.C / V;
+    const int tid = threadIdx.x, chunk = blockIdx.x, b = blockIdx.z;
+    const Place l = Place::of<V>(p, blockIdx.y, b, tid, GN_T);
     const int r0 = chunk * p.rows, r1 = min(p.n, r0 + p.rows);
-    const T* X = (const T*)p.x + (size_t)b * p.n * p.ldx;
-    const T* DY = (const T*)p.dy + (size_t)b * p.n * p.ldy;
-    float2* out = p.cpart + ((size_t)b * p.chunks + chunk) * p.C;
+    const T* X = (const T*)p.x + (size_t)b * p.n * p.ldx + l.ch0;
+    const T* DY = (const T*)p.dy + (size_t)b * p.n * p.ldy + l.ch0;
+    float2* out = p.cpart + ((size_t)b * p.chunks + chunk) * p.C + l.ch0;
     const bool silu = p.act == UWIR_ACT_SILU;
-    constexpr int R = GN_R / 2;
-    for (int c0 = 0; c0 < nv; c0 += GN_T) {
-        const int tw = min(nv - c0, GN_T), RL = GN_T / tw, cv = tid % tw, rl = tid / tw;
-        const int cb = (c0 + cv) * V;
+    for (int v0 = 0; v0 < l.tw; v0 += GN_T) {
+        const bool wide = l.tw > GN_T;
+        const int cv = wide ? v0 + tid : l.cv;
         float s1[V], s2[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) s1[j] = s2[j] = 0.f;
-        if (rl < RL) {
-            BwdCoef<V> co;
-            co.load(p, b, cb);
-            for (int r = r0 + rl; r < r1; r += RL * R) {
-                Pack<T, V> bx[R], bd[R];
-                const int k = min(R, (r1 - r + RL - 1) / RL);
+        if (wide ? cv < l.tw : l.rl < l.RL) {
+            Coef<V> co;
+            bwd_stats<V, T>(p, co, b, l.ch0 + cv * V);
+            row_batches<GN_RB>(r0 + (wide ? 0 : l.rl), r1, l.RL, [&](int r, int k) {
+                Pack<T, V> bx[GN_RB], bd[GN_RB];
+                load_rows<GN_RB>(bx, X + cv * V, p.ldx, r, l.RL, k);
+                load_rows<GN_RB>(bd, DY + cv * V, p.ldy, r, l.RL, k);
+                bwd_batch<GN_RB>(bx, bd, co, k, silu, s1, s2);
+            });
 #pragma unroll
-                for (int i = 0; i < R; ++i) {
-                    const size_t row = i < k ? r + i * RL : r;
-                    bx[i].load(X + row * p.ldx + cb);
-                    bd[i].load(DY + row * p.ldy + cb);
-                }
+            for (int j = 0; j < V; ++j) s2[j] *= co.r[j];
+        }
+        if (wide) {
+            if (cv < l.tw)
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    float t1 = 0.f, t2 = 0.f;   // a short chain per batch keeps the fp32 sums close to pairwise
-#pragma unroll
-                    for (int i = 0; i < R; ++i)
-                        if (i < k) {
-                            float dz, xh;
-                            co.grad(j, bx[i].get(j), bd[i].get(j), silu, dz, xh);
-                            t1 += dz;
-                            t2 = fmaf(dz, xh, t2);
-                        }
-                    s1[j] += t1;
-                    s2[j] += t2;
-                }
-            }
+                for (int j = 0; j < V; ++j) out[cv * V + j] = make_float2(s1[j], s2[j]);
+            continue;
         }
 #pragma unroll
         for (int j = 0; j < V; ++j) red[tid * V + j] = make_float2(s1[j], s2[j]);
         __syncthreads();
-        for (int c = tid; c < tw * V; c += GN_T) {
+        // a team of T / width threads per channel (a power of two within a wave) over the row lanes
+        int team = 1;
+        while (team < 64 && team * 2 * l.sc <= GN_T) team *= 2;
+        for (int c0 = 0; c0 < l.sc; c0 += GN_T / team) {
+            const int c = c0 + tid / team;
             double a = 0., q = 0.;
-            for (int l = 0; l < RL; ++l) {
-                const float2 v = red[l * tw * V + c];
-                a += v.x;
-                q += v.y;
+            if (c < l.sc)
+                for (int i = tid & (team - 1); i < l.RL; i += team) {
+                    const float2 v = red[i * l.sc + c];
+                    a += v.x;
+                    q += v.y;
+                }
+            for (int o = team >> 1; o; o >>= 1) {
+                a += shfl_xor_d(a, o);
+                q += shfl_xor_d(q, o);
             }
-            out[c0 * V + c] = make_float2((float)a, (float)q);
+            if (c < l.sc && (tid & (team - 1)) == 0) out[c] = make_float2((float)a, (float)q);
         }
-        __syncthreads();
     }
 }
 
-// S1, S2 of 64 channels of one image: 4 lanes a channel over the chunks; the modulation's gradient falls out here
+// sums over the chunks of 64 channels of one image, 8 lanes a channel: ahead of the output pass where a slab's partials are
+// too many for every output block to read
 __global__ void __launch_bounds__(GN_T) gn_bwd_reduce_kernel(GnArgs p) {
-    __shared__ double2 red[4][64];
+    __shared__ double2 red[8][64];
     const int cl = threadIdx.x & 63, l = threadIdx.x >> 6, c = blockIdx.x * 64 + cl, b = blockIdx.y;
     double a = 0., q = 0.;
     if (c < p.C)
-        for (int i = l; i < p.chunks; i += 4) {
+        for (int i = l; i < p.chunks; i += 8) {
             const float2 v = p.cpart[((size_t)b * p.chunks + i) * p.C + c];
             a += v.x;
             q += v.y;
@@ -412,33 +513,31 @@ __global__ void __launch_bounds__(GN_T) gn_bwd_reduce_kernel(GnArgs p) {
     red[l][cl] = make_double2(a, q);
     __syncthreads();
     if (l == 0 && c < p.C) {
-        for (int i = 1; i < 4; ++i) {
+        for (int i = 1; i < 8; ++i) {
             a += red[i][cl].x;
             q += red[i][cl].y;
         }
         p.csum[(size_t)b * p.C + c] = make_float2((float)a, (float)q);
-        if (p.dss) {
-            p.dss[(size_t)b * p.ld_dss + c] = (float)(p.gamma[c] * q + p.beta[c] * a);
-            p.dss[(size_t)b * p.ld_dss + p.C + c] = (float)a;
-        }
     }
 }
 
-// dgamma, dbeta of 64 channels: 4 lanes a channel over the images
+// dgamma, dbeta of 64 channels: 8 lanes a channel over the images (and their chunks)
 __device__ __forceinline__ void affine_grads(const GnArgs& p, int tile, double2 (*red)[64]) {
     const int cl = threadIdx.x & 63, l = threadIdx.x >> 6, c = tile * 64 + cl;
     double dg = 0., db = 0.;
     if (c < p.C)
-        for (int b = l; b < p.B; b += 4) {
-            const float2 v = p.csum[(size_t)b * p.C + c];
+        for (int b = l; b < p.B; b += 8) {
             const double f = p.ss ? 1. + (double)p.ss[(size_t)b * p.ld_ss + c] : 1.;
-            dg += f * v.y;
-            db += f * v.x;
+            for (int i = 0; i < p.sum_chunks; ++i) {
+                const float2 v = p.sums[((size_t)b * p.sum_chunks + i) * p.C + c];
+                dg += f * v.y;
+                db += f * v.x;
+            }
         }
     red[l][cl] = make_double2(dg, db);
     __syncthreads();
     if (l == 0 && c < p.C) {
-        for (int i = 1; i < 4; ++i) {
+        for (int i = 1; i < 8; ++i) {
             dg += red[i][cl].x;
             db += red[i][cl].y;
         }
@@ -448,182 +547,166 @@ __device__ __forceinline__ void affine_grads(const GnArgs& p, int tile, double2 
 }
 
 __global__ void __launch_bounds__(GN_T) gn_bwd_affine_kernel(GnArgs p) {
-    __shared__ double2 red[4][64];
+    __shared__ double2 red[8][64];
     affine_grads(p, blockIdx.x, red);
 }
 
-// dx = r (w dz - m1 - xh m2); the last row of blocks (b == B) forms dgamma, dbeta instead
+// the modulation's gradient of one channel
+__device__ __forceinline__ void put_dss(const GnArgs& p, int b, int c, double s1, double s2) {
+    if (!p.dss) return;
+    p.dss[(size_t)b * p.ld_dss + c] = (float)(p.gamma[c] * s2 + p.beta[c] * s1);
+    p.dss[(size_t)b * p.ld_dss + p.C + c] = (float)s1;
+}
+
+// output pass; the last row of blocks (b == B) forms dgamma, dbeta instead
 template <typename T, int V>
-__global__ void __launch_bounds__(GN_T) gn_bwd_apply_kernel(GnArgs p) {
+__global__ void __launch_bounds__(GN_T, 4) gn_bwd_apply_kernel(GnArgs p) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    const int tid = threadIdx.x, chunk = blockIdx.x, b = blockIdx.y;
+    const int tid = threadIdx.x, chunk = blockIdx.x, b = blockIdx.z;
     if (b == p.B) {
-        for (int t = chunk; t * 64 < p.C; t += gridDim.x) {
+        for (int t = chunk + blockIdx.y * gridDim.x; t * 64 < p.C; t += gridDim.x * gridDim.y) {
             affine_grads(p, t, reinterpret_cast<double2(*)[64]>(smem));
             __syncthreads();
         }
         return;
     }
-    float2* gm = reinterpret_cast<float2*>(smem);   // [G] (m1, m2)
-    const int nv = p.C / V, cg = p.cg;
-    const double N = (double)p.n * cg;
-    group_sums(p.G, cg, tid, GN_T,
-               [&](int g, int i) {
-                   const int c = g * cg + i;
-                   const float2 v = p.csum[(size_t)b * p.C + c];
-                   const double w = (double)p.gamma[c] * (p.ss ? 1. + (double)p.ss[(size_t)b * p.ld_ss + c] : 1.);
-                   return make_double2(w * v.x, w * v.y);
-               },
-               [&](int g, double s, double q) { gm[g] = make_float2((float)(s / N), (float)(q / N)); });
-    __syncthreads();
+    double2* scratch = reinterpret_cast<double2*>(smem);            // [GN_T / 64]
+    double2* ch = scratch + GN_T / 64;                              // [slab] w (S1, S2)
+    float2* gm = reinterpret_cast<float2*>(ch + p.slab);            // [slab / cg] (m1, m2)
+    const Place l = Place::of<V>(p, blockIdx.y, b, tid, GN_T);
+    const int cg = p.cg;
     const int r0 = chunk * p.rows, r1 = min(p.n, r0 + p.rows);
-    const T* X = (const T*)p.x + (size_t)b * p.n * p.ldx;
-    const T* DY = (const T*)p.dy + (size_t)b * p.n * p.ldy;
-    T* DX = (T*)p.out + (size_t)b * p.n * p.ldo;
-    const bool silu = p.act == UWIR_ACT_SILU;
-    constexpr int R = GN_R / 2;
-    for (int c0 = 0; c0 < nv; c0 += GN_T) {
-        const int tw = min(nv - c0, GN_T), RL = GN_T / tw, cv = tid % tw, rl = tid / tw;
-        if (rl >= RL) continue;
-        const int cb = (c0 + cv) * V;
-        BwdCoef<V> co;
-        co.load(p, b, cb);
-        float m1[V], m2[V];
+    const T* X = (const T*)p.x + (size_t)b * p.n * p.ldx + l.ch0;
+    const T* DY = (const T*)p.dy + (size_t)b * p.n * p.ldy + l.ch0;
+    T* DX = (T*)p.out + (size_t)b * p.n * p.ldo + l.ch0;
+    const bool silu = p.act == UWIR_ACT_SILU, wide = l.tw > GN_T;
+    for (int c = tid; c < l.sc; c += GN_T) {
+        double a = 0., q = 0.;
+        const float2* src = p.sums + (size_t)b * p.sum_chunks * p.C + l.ch0 + c;
+#pragma unroll 8
+        for (int i = 0; i < p.sum_chunks; ++i) {
+            const float2 v = src[(size_t)i * p.C];
+            a += v.x;
+            q += v.y;
+        }
+        const int cc = l.ch0 + c;
+        const double w = (double)p.gamma[cc] * (p.ss ? 1. + (double)p.ss[(size_t)b * p.ld_ss + cc] : 1.);
+        ch[c] = make_double2(w * a, w * q);
+        if (chunk == 0) put_dss(p, b, cc, a, q);
+    }
+    __syncthreads();
+    group_sums<GN_T>(l.sc / cg, cg, tid, scratch, [&](int g, int i) { return ch[g * cg + i]; },
+                     [&](int g, double s, double q) { gm[g] = make_float2((float)(s * p.inv_n), (float)(q * p.inv_n)); });
+    auto walk = [&](int cv, int r, int step) {
+        Coef<V> co;
+        float u1[V], u2[V];
+        bwd_stats<V, T>(p, co, b, l.ch0 + cv * V);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const float2 g = gm[(cb + j) / cg];
-            m1[j] = co.r[j] * g.x;
-            m2[j] = co.r[j] * g.y;
+            const float2 g = gm[wide ? 0 : (cv * V + j) / cg];
+            u1[j] = co.r[j] * g.x;
+            u2[j] = co.r[j] * co.r[j] * g.y;
         }
-        for (int r = r0 + rl; r < r1; r += RL * R) {
-            Pack<T, V> bx[R], bd[R];
-            const int k = min(R, (r1 - r + RL - 1) / RL);
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-                const size_t row = i < k ? r + i * RL : r;
-                bx[i].load(X + row * p.ldx + cb);
-                bd[i].load(DY + row * p.ldy + cb);
-            }
-#pragma unroll
-            for (int i = 0; i < R; ++i)
-                if (i < k) {
-                    Pack<T, V> o;
-#pragma unroll
-                    for (int j = 0; j < V; ++j) {
-                        float dz, xh;
-                        co.grad(j, bx[i].get(j), bd[i].get(j), silu, dz, xh);
-                        o.set(j, fmaf(co.a[j], dz, -fmaf(xh, m2[j], m1[j])));   // a = r w
-                    }
-                    o.store(DX + (size_t)(r + i * RL) * p.ldo + cb);
-                }
-        }
-    }
+        row_batches<GN_RB>(r, r1, step, [&](int r, int k) {
+            Pack<T, V> bx[GN_RB], bd[GN_RB];
+            load_rows<GN_RB>(bx, X + cv * V, p.ldx, r, step, k);
+            load_rows<GN_RB>(bd, DY + cv * V, p.ldy, r, step, k);
+            bwd_emit<GN_RB>(bx, bd, co, u1, u2, DX + cv * V, p.ldo, r, step, k, silu);
+        });
+    };
+    if (wide)
+        for (int cv = tid; cv < l.tw; cv += GN_T) walk(cv, r0, 1);
+    else if (l.rl < l.RL)
+        walk(l.cv, r0 + l.rl, l.RL);
 }
 
-// ---------------------------------------------------------------------------------------- backward, resident
 template <typename T, int V, int TH>
 __global__ void __launch_bounds__(TH) gn_bwd_resident_kernel(GnArgs p) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     float2* red = reinterpret_cast<float2*>(smem);                     // [TH][V]
-    double2* ch = reinterpret_cast<double2*>(red + TH * V);            // [slab] w (S1, S2)
+    double2* scratch = reinterpret_cast<double2*>(red + TH * V);       // [TH / 64]
+    double2* ch = scratch + TH / 64;                                   // [slab] w (S1, S2)
     float2* gm = reinterpret_cast<float2*>(ch + p.slab);               // [slab / cg]
     const int tid = threadIdx.x, b = blockIdx.y, cg = p.cg;
-    const int ch0 = blockIdx.x * p.slab, sc = min(p.slab, p.C - ch0), gs = sc / cg;
-    const int tw = sc / V, RL = TH / tw, cv = tid % tw, rl = tid / tw, cb = ch0 + cv * V;
+    const Place l = Place::of<V>(p, blockIdx.x, b, tid, TH);
+    const int cb = l.ch0 + l.cv * V;
     const T* X = (const T*)p.x + (size_t)b * p.n * p.ldx + cb;
     const T* DY = (const T*)p.dy + (size_t)b * p.n * p.ldy + cb;
     const bool silu = p.act == UWIR_ACT_SILU;
-    const int k = rl < RL && rl < p.n ? (p.n - rl + RL - 1) / RL : 0;
+    const int k = l.rl < l.RL && l.rl < p.n ? (p.n - l.rl + l.RL - 1) / l.RL : 0;
     Pack<T, V> bx[GN_R], bd[GN_R];
-    BwdCoef<V> co;
+    Coef<V> co;
     float s1[V], s2[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) s1[j] = s2[j] = 0.f;
     if (k > 0) {
+        load_rows<GN_R>(bx, X, p.ldx, l.rl, l.RL, k);
+        load_rows<GN_R>(bd, DY, p.ldy, l.rl, l.RL, k);
+        bwd_stats<V, T>(p, co, b, cb);
+        bwd_batch<GN_R>(bx, bd, co, k, silu, s1, s2);
 #pragma unroll
-        for (int i = 0; i < GN_R; ++i) {
-            const size_t row = i < k ? rl + i * RL : rl;
-            bx[i].load(X + row * p.ldx);
-            bd[i].load(DY + row * p.ldy);
-        }
-        co.load(p, b, cb);
-#pragma unroll
-        for (int i = 0; i < GN_R; ++i)
-            if (i < k) {
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    float dz, xh;
-                    co.grad(j, bx[i].get(j), bd[i].get(j), silu, dz, xh);
-                    s1[j] += dz;
-                    s2[j] = fmaf(dz, xh, s2[j]);
-                }
-            }
+        for (int j = 0; j < V; ++j) s2[j] *= co.r[j];
     }
 #pragma unroll
     for (int j = 0; j < V; ++j) red[tid * V + j] = make_float2(s1[j], s2[j]);
     __syncthreads();
-    const int rows = min(RL, p.n);
-    for (int c = tid; c < sc; c += TH) {
+    const int rows = min(l.RL, p.n);
+    int team = 1;
+    while (team < 64 && team * 2 * l.sc <= TH) team *= 2;
+    for (int c0 = 0; c0 < l.sc; c0 += TH / team) {
+        const int c = c0 + tid / team;
         double a = 0., q = 0.;
-        for (int l = 0; l < rows; ++l) {
-            const float2 v = red[l * sc + c];
-            a += v.x;
-            q += v.y;
+        if (c < l.sc)
+            for (int i = tid & (team - 1); i < rows; i += team) {
+                const float2 v = red[i * l.sc + c];
+                a += v.x;
+                q += v.y;
+            }
+        for (int o = team >> 1; o; o >>= 1) {
+            a += shfl_xor_d(a, o);
+            q += shfl_xor_d(q, o);
         }
-        const int cc = ch0 + c;
-        const double ga = p.gamma[cc], f = p.ss ? 1. + (double)p.ss[(size_t)b * p.ld_ss + cc] : 1.;
-        ch[c] = make_double2(ga * f * a, ga * f * q);
-        if (p.dss) {
-            p.dss[(size_t)b * p.ld_dss + cc] = (float)(ga * q + p.beta[cc] * a);
-            p.dss[(size_t)b * p.ld_dss + p.C + cc] = (float)a;
-        }
-        if (p.B == 1) {   // nothing to sum over: the affine's gradient is complete
-            p.dgamma[cc] = (float)(f * q);
-            p.dbeta[cc] = (float)(f * a);
-        } else {
-            p.csum[(size_t)b * p.C + cc] = make_float2((float)a, (float)q);
+        if (c < l.sc && (tid & (team - 1)) == 0) {
+            const int cc = l.ch0 + c;
+            const double f = p.ss ? 1. + (double)p.ss[(size_t)b * p.ld_ss + cc] : 1., w = f * p.gamma[cc];
+            ch[c] = make_double2(w * a, w * q);
+            put_dss(p, b, cc, a, q);
+            if (p.B == 1) {   // nothing to sum over: the affine's gradient is complete
+                p.dgamma[cc] = (float)(f * q);
+                p.dbeta[cc] = (float)(f * a);
+            } else {
+                p.csum[(size_t)b * p.C + cc] = make_float2((float)a, (float)q);
+            }
         }
     }
     __syncthreads();
-    const double N = (double)p.n * cg;
-    group_sums(gs, cg, tid, TH, [&](int g, int i) { return ch[g * cg + i]; },
-               [&](int g, double s, double q) { gm[g] = make_float2((float)(s / N), (float)(q / N)); });
-    __syncthreads();
+    group_sums<TH>(l.sc / cg, cg, tid, scratch, [&](int g, int i) { return ch[g * cg + i]; },
+                   [&](int g, double s, double q) { gm[g] = make_float2((float)(s * p.inv_n), (float)(q * p.inv_n)); });
     if (k <= 0) return;
-    T* DX = (T*)p.out + (size_t)b * p.n * p.ldo + cb;
-    float m1[V], m2[V];
+    float u1[V], u2[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const float2 g = gm[(cv * V + j) / cg];
-        m1[j] = co.r[j] * g.x;
-        m2[j] = co.r[j] * g.y;
+        const float2 g = gm[(l.cv * V + j) / cg];
+        u1[j] = co.r[j] * g.x;
+        u2[j] = co.r[j] * co.r[j] * g.y;
     }
-#pragma unroll
-    for (int i = 0; i < GN_R; ++i)
-        if (i < k) {
-            Pack<T, V> o;
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                float dz, xh;
-                co.grad(j, bx[i].get(j), bd[i].get(j), silu, dz, xh);
-                o.set(j, fmaf(co.a[j], dz, -fmaf(xh, m2[j], m1[j])));
-            }
-            o.store(DX + (size_t)(rl + i * RL) * p.ldo);
-        }
+    bwd_emit<GN_R>(bx, bd, co, u1, u2, (T*)p.out + (size_t)b * p.n * p.ldo + cb, p.ldo, l.rl, l.RL, k, silu);
 }
 
 // ---------------------------------------------------------------------------------------- launch rules
 int gcd_i(int a, int b) { return b ? gcd_i(b, a % b) : a; }
 
-// channels a block of the resident form owns: whole groups and whole vectors, at least 64 bytes of a row
-int slab_channels(int C, int cg, int V, int es) {
+// channels a block owns: whole groups and whole vectors, at least `bytes` of a row
+int slab_channels(int C, int cg, int V, int es, int bytes) {
     const int unit = cg / gcd_i(cg, V) * V;
     int s = unit;
-    while (s * es < 64 && s < C) s += unit;
+    while (s * es < bytes && s < C) s += unit;
     return s < C ? s : C;
 }
 
-size_t resident_lds(int T, int slab, int cg, int V) { return (size_t)T * V * 8 + (size_t)slab * 16 + (size_t)(slab / cg) * 8; }
+size_t resident_lds(int T, int slab, int cg, int V) {
+    return (size_t)T * V * 8 + (size_t)T / 64 * 16 + (size_t)slab * 16 + (size_t)(slab / cg) * 8;
+}
 
 // threads of the resident form (0: the slab's rows do not fit the registers of a block, or its sums 64 KB of LDS)
 int resident_threads(int n, int slab, int cg, int V) {
@@ -633,14 +716,22 @@ int resident_threads(int n, int slab, int cg, int V) {
     return 0;
 }
 
-int stream_chunks(int B, int n) {
-    int c = 1024 / (B > 0 ? B : 1);
+// row chunks of the streamed form: two blocks per CU over the whole launch, a batch of rows a thread at least.  An upper bound
+// over the slab widths (any vector width), so that the workspace's size does not depend on alignment.
+int stream_chunks(int B, int n, int slabs) {
+    long long c = 512 / ((long long)B * slabs);
     c = c < 1 ? 1 : (c > GN_MAX_CHUNKS ? GN_MAX_CHUNKS : c);
-    const int most = ceil_div(n, 8);   // a chunk has a batch of rows at least
-    return c < most ? c : most;
+    const int most = ceil_div(n, 16);
+    return c < most ? (int)c : most;
 }
 
 size_t al256(size_t v) { return (v + 255) & ~(size_t)255; }
+
+// a slab of more vectors than a block has threads must be a single group (the kernels' wide path)
+bool slab_ok(int C, int cg, int V, int es) {
+    const int s = slab_channels(C, cg, V, es, 128);
+    return s / V <= GN_T || s == cg;
+}
 
 bool vec_ok(const void* p, size_t ld, int V, int es) {
     const size_t a = (size_t)V * es > 16 ? 16 : (size_t)V * es;
@@ -656,9 +747,15 @@ template <typename F> int with_v(int V, F f) {
     }
 }
 
+void stream_shape(GnArgs& p, int V, int es) {
+    p.slab = slab_channels(p.C, p.cg, V, es, 128);
+    p.chunks = stream_chunks(p.B, p.n, ceil_div(p.C, p.slab));
+    p.rows = ceil_div(p.n, p.chunks);
+}
+
 template <typename TX, typename TO, int V> void launch_fwd(GnArgs p, hipStream_t st) {
     const int es = sizeof(TX);
-    p.slab = slab_channels(p.C, p.cg, V, es);
+    p.slab = slab_channels(p.C, p.cg, V, es, 64);
     const int T = resident_threads(p.n, p.slab, p.cg, V);
     if (T) {
         const size_t lds = resident_lds(T, p.slab, p.cg, V);
@@ -669,19 +766,21 @@ template <typename TX, typename TO, int V> void launch_fwd(GnArgs p, hipStream_t
             hipLaunchKernelGGL((gn_resident_kernel<TX, TO, V, 512>), grid, dim3(512), lds, st, p);
         return;
     }
-    p.chunks = stream_chunks(p.B, p.n);
-    p.rows = ceil_div(p.n, p.chunks);
-    const dim3 grid(p.chunks, p.B);
-    hipLaunchKernelGGL((gn_stats_kernel<TX, V>), grid, dim3(GN_T), (size_t)GN_T * V * 8 + (size_t)p.C * 16, st, p);
-    hipLaunchKernelGGL((gn_apply_kernel<TX, TO, V>), grid, dim3(GN_T), (size_t)p.G * 8, st, p);
+    stream_shape(p, V, es);
+    const dim3 grid(p.chunks, ceil_div(p.C, p.slab), p.B);
+    const size_t scratch = GN_T / 64 * 16;
+    hipLaunchKernelGGL((gn_stats_kernel<TX, V>), grid, dim3(GN_T), scratch + (size_t)GN_T * (V > 2 ? V : 2) * 8, st, p);
+    hipLaunchKernelGGL((gn_apply_kernel<TX, TO, V>), grid, dim3(GN_T), scratch + (size_t)(p.slab / p.cg) * 8, st, p);
 }
 
 template <typename T, int V> void launch_bwd(GnArgs p, hipStream_t st) {
-    p.slab = slab_channels(p.C, p.cg, V, sizeof(T));
+    p.slab = slab_channels(p.C, p.cg, V, sizeof(T), 64);
     const int TH = resident_threads(p.n, p.slab, p.cg, V);
     if (TH) {
         const size_t lds = resident_lds(TH, p.slab, p.cg, V);
         const dim3 grid(ceil_div(p.C, p.slab), p.B);
+        p.sums = p.csum;
+        p.sum_chunks = 1;
         if (TH == 256)
             hipLaunchKernelGGL((gn_bwd_resident_kernel<T, V, 256>), grid, dim3(256), lds, st, p);
         else
@@ -689,12 +788,19 @@ template <typename T, int V> void launch_bwd(GnArgs p, hipStream_t st) {
         if (p.B > 1) hipLaunchKernelGGL(gn_bwd_affine_kernel, dim3(ceil_div(p.C, 64)), dim3(GN_T), 0, st, p);
         return;
     }
-    p.chunks = stream_chunks(p.B, p.n);
-    p.rows = ceil_div(p.n, p.chunks);
-    hipLaunchKernelGGL((gn_bwd_sums_kernel<T, V>), dim3(p.chunks, p.B), dim3(GN_T), (size_t)GN_T * V * 8, st, p);
-    hipLaunchKernelGGL(gn_bwd_reduce_kernel, dim3(ceil_div(p.C, 64), p.B), dim3(GN_T), 0, st, p);
-    const size_t lds = (size_t)p.G * 8 > 4096 ? (size_t)p.G * 8 : 4096;
-    hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V>), dim3(p.chunks, p.B + 1), dim3(GN_T), lds, st, p);
+    stream_shape(p, V, sizeof(T));
+    const int slabs = ceil_div(p.C, p.slab);
+    hipLaunchKernelGGL((gn_bwd_sums_kernel<T, V>), dim3(p.chunks, slabs, p.B), dim3(GN_T), (size_t)GN_T * V * 8, st, p);
+    p.sums = p.cpart;
+    p.sum_chunks = p.chunks;
+    if (p.slab * p.chunks > 8192) {   // 64 KB of partials a block: sum them once instead
+        hipLaunchKernelGGL(gn_bwd_reduce_kernel, dim3(ceil_div(p.C, 64), p.B), dim3(GN_T), 0, st, p);
+        p.sums = p.csum;
+        p.sum_chunks = 1;
+    }
+    size_t lds = GN_T / 64 * 16 + (size_t)p.slab * 16 + (size_t)(p.slab / p.cg) * 8;
+    if (lds < 8 * 64 * 16) lds = 8 * 64 * 16;
+    hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V>), dim3(p.chunks, slabs, p.B + 1), dim3(GN_T), lds, st, p);
 }
 
 bool overlaps(const void* a, size_t na, const void* b, size_t nb) {
@@ -729,7 +835,7 @@ int check_common(const char* what, int B, int n, int C, int G, int act, size_t w
 // partials of the streamed form: per chunk and group (forward) or per chunk and channel (backward), and per image and channel
 extern "C" size_t uwir_group_norm_act_workspace_bytes(int B, int n, int C, int groups) {
     if (B <= 0 || n <= 0 || C <= 0 || groups <= 0) return 0;
-    const size_t ch = stream_chunks(B, n);
+    const size_t ch = stream_chunks(B, n, 1);   // fewer with several slabs
     const size_t fwd = (size_t)B * ch * groups * 16, bwd = al256((size_t)B * ch * C * 8) + (size_t)B * C * 8;
     return al256(fwd > bwd ? fwd : bwd);
 }
@@ -755,10 +861,10 @@ extern "C" int uwir_group_norm_act(const void* x, int x_dtype, size_t ldx, int B
     p.x = x; p.out = out; p.gamma = gamma; p.beta = beta; p.ss = scale_shift; p.mean = mean; p.rstd = rstd;
     p.part = (double2*)workspace;
     p.ldx = ldx; p.ldo = ldo; p.ld_ss = ld_ss;
-    p.B = B; p.n = n; p.C = C; p.G = groups; p.cg = C / groups; p.eps = eps; p.act = act;
+    p.B = B; p.n = n; p.C = C; p.G = groups; p.cg = C / groups; p.eps = eps; p.act = act; p.inv_n = 1. / ((double)n * p.cg);
     // widest vector (16 bytes of x at most) that the channel count, strides and addresses allow
     int V = 16 / ex;
-    while (V > 1 && (C % V || !vec_ok(x, ldx, V, ex) || !vec_ok(out, ldo, V, eo))) V >>= 1;
+    while (V > 1 && (C % V || !slab_ok(C, p.cg, V, ex) || !vec_ok(x, ldx, V, ex) || !vec_ok(out, ldo, V, eo))) V >>= 1;
     hipStream_t st = (hipStream_t)stream;
     with_v(V, [&](auto v) {
         constexpr int W = decltype(v)::value;
@@ -801,11 +907,11 @@ extern "C" int uwir_group_norm_act_backward(const void* dy, size_t ldy, const vo
     p.x = x; p.dy = dy; p.out = dx; p.gamma = gamma; p.beta = beta; p.ss = scale_shift; p.mean_in = mean; p.rstd_in = rstd;
     p.dgamma = dgamma; p.dbeta = dbeta; p.dss = dscale_shift;
     p.ldx = ldx; p.ldy = ldy; p.ldo = ldd; p.ld_ss = ld_ss; p.ld_dss = ld_dss;
-    p.B = B; p.n = n; p.C = C; p.G = groups; p.cg = C / groups; p.act = act;
+    p.B = B; p.n = n; p.C = C; p.G = groups; p.cg = C / groups; p.act = act; p.inv_n = 1. / ((double)n * p.cg);
     p.cpart = (float2*)workspace;
-    p.csum = (float2*)((char*)workspace + al256((size_t)B * stream_chunks(B, n) * C * 8));
+    p.csum = (float2*)((char*)workspace + al256((size_t)B * stream_chunks(B, n, 1) * C * 8));
     int V = 16 / es;
-    while (V > 1 && (C % V || !vec_ok(x, ldx, V, es) || !vec_ok(dy, ldy, V, es) || !vec_ok(dx, ldd, V, es))) V >>= 1;
+    while (V > 1 && (C % V || !slab_ok(C, p.cg, V, es) || !vec_ok(x, ldx, V, es) || !vec_ok(dy, ldy, V, es) || !vec_ok(dx, ldd, V, es))) V >>= 1;
     hipStream_t st = (hipStream_t)stream;
     with_v(V, [&](auto v) {
         constexpr int W = decltype(v)::value;

@@ -19,12 +19,12 @@ def _stream(t) -> int:
     operand (tensor or device) of the op: the library launches in the current HIP device context, so an operand on
     another GPU is an error here (it used to enqueue on the wrong GPU's stream silently).  The module-level entry
     points (student / UNet / DA-CLIP / sampler forwards) make their input's device current themselves."""
-    s = torch.cuda.current_stream()
     dev = t.device if isinstance(t, torch.Tensor) else t
-    if dev.type != "cuda" or (dev.index is not None and dev.index != s.device_index):
-        raise ValueError(f"operand on {dev} but the current HIP device is cuda:{s.device_index}: run under "
-                         f"torch.cuda.device(...) (the model-level forwards do)")
-    return s.cuda_stream
+    cur = torch._C._cuda_getDevice() if dev.type == "cuda" else None   # what torch.cuda.current_stream() asks, without its
+    if cur is None or (dev.index is not None and dev.index != cur):     # Stream object: 3 us a launch
+        raise ValueError(f"operand on {dev} but the current HIP device is {'not asked' if cur is None else f'cuda:{cur}'}: run "
+                         f"under torch.cuda.device(...) (the model-level forwards do)")
+    return torch._C._cuda_getCurrentRawStream(cur)
 
 
 def on_operand_device(fn):
@@ -347,45 +347,44 @@ def flash_attn(q, k, v1, v2, B: int, n: int, heads: int, hd: int, scale: float, 
         _TIMING["events"].append((("flash_attn", B, n, heads, hd, 1 if v2 is None else 2, dt), ev0, ev1))
 
 
-def _operands(what: str, first: torch.Tensor, *ts) -> None:
-    """Every given tensor on one GPU: a kernel follows raw pointers, whatever device they belong to."""
-    for t in ts:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"{what}: operands on {first.device} and {t.device}")
+def _mat(what: str, name: str, t: torch.Tensor, rows: int, cols: int, dtype: torch.dtype, dev: int) -> int:
+    """Check a [rows, cols] view with unit inner stride, of `dtype` on GPU `dev` (a kernel follows raw pointers, whatever device
+    they belong to) -> its row stride; of a single row, whose stride means nothing, cols.  Runs on every call, next to launches
+    of a few microseconds: one query each of shape, stride, type and device."""
+    ld, inner = t.stride() if t.dim() == 2 else (0, 0)
+    if t.shape != (rows, cols) or (inner != 1 and cols > 1):
+        raise ValueError(f"{what}: {name} must be a [{rows}, {cols}] view with unit inner stride, got {tuple(t.shape)} / {t.stride()}")
+    if t.dtype is not dtype:
+        raise TypeError(f"{what}: {name} must be {dtype}, got {t.dtype}")
+    if t.get_device() != dev:
+        raise ValueError(f"{what}: {name} is on {t.device}, not with the other operands")
+    return ld if rows > 1 else max(cols, 1)
 
 
-def _rows_cols(what: str, name: str, t: torch.Tensor, rows: int, cols: int) -> None:
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols or (t.stride(1) != 1 and cols > 1):
-        raise ValueError(f"{what}: {name} must be a [{rows}, {cols}] view with unit inner stride, got {tuple(t.shape)}")
-
-
-def _row_stride(t: torch.Tensor) -> int:
-    """Row stride of a 2-D view; of a single row (whose stride means nothing) its width."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
-
-
-def _vector(what: str, name: str, t: Optional[torch.Tensor], *shape) -> None:
-    if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous()):
+def _vec(what: str, name: str, t: torch.Tensor, shape: tuple, dev: int) -> int:
+    """Check a contiguous fp32 tensor on GPU `dev` -> its address."""
+    if t.shape != shape or t.dtype is not torch.float32 or not t.is_contiguous():
         raise ValueError(f"{what}: {name} must be a contiguous fp32 {list(shape)}")
+    if t.get_device() != dev:
+        raise ValueError(f"{what}: {name} is on {t.device}, not with the other operands")
+    return t.data_ptr()
+
+
+def _scratch(what: str, t: torch.Tensor, dev: int) -> int:
+    if not t.is_contiguous() or t.get_device() != dev:
+        raise ValueError(f"{what}: workspace must be contiguous and with the other operands")
+    return t.nbytes
 
 
 def group_norm_act_workspace_bytes(B: int, n: int, C_: int, groups: int) -> int:
     return int(_lib.load().uwir_group_norm_act_workspace_bytes(B, n, C_, groups))
 
 
-def _gn_check(what, x, B, n, C_, groups, gamma, beta, act, scale_shift, workspace):
+def _gn_check(what, B, n, C_, groups, act) -> None:
     if B < 1 or n < 1 or C_ < 1 or groups < 1 or C_ % groups:
         raise ValueError(f"{what}: need B, n, C > 0 and groups dividing C")
-    if act not in (ACT_NONE, ACT_SILU):
+    if act != ACT_NONE and act != ACT_SILU:
         raise ValueError(f"{what}: act must be ACT_NONE or ACT_SILU")
-    _rows_cols(what, "x", x, B * n, C_)
-    _vector(what, "gamma", gamma, C_)
-    _vector(what, "beta", beta, C_)
-    if scale_shift is not None:
-        _f32(scale_shift)
-        _rows_cols(what, "scale_shift", scale_shift, B, 2 * C_)
-    if not workspace.is_contiguous():
-        raise ValueError(f"{what}: workspace must be contiguous")
 
 
 def group_norm_act(x: torch.Tensor, B: int, n: int, C_: int, groups: int, eps: float, gamma: torch.Tensor, beta: torch.Tensor,
@@ -395,15 +394,18 @@ def group_norm_act(x: torch.Tensor, B: int, n: int, C_: int, groups: int, eps: f
     be x).  ``scale_shift`` [B, 2C] = [scale | shift] per image.  ``mean`` / ``rstd`` [B, groups] keep the statistics for
     ``group_norm_act_backward``.  workspace: group_norm_act_workspace_bytes, any contiguous tensor; see uwir_group_norm_act."""
     what = "group_norm_act"
-    _gn_check(what, x, B, n, C_, groups, gamma, beta, act, scale_shift, workspace)
-    _rows_cols(what, "out", out, B * n, C_)
-    _vector(what, "mean", mean, B, groups)
-    _vector(what, "rstd", rstd, B, groups)
-    _operands(what, x, gamma, beta, out, workspace, scale_shift, mean, rstd)
-    _lib.check(_lib.load().uwir_group_norm_act(
-        _p(x), _dt(x), _row_stride(x), B, n, C_, groups, eps, _p(gamma), _p(beta), _p(scale_shift),
-        0 if scale_shift is None else _row_stride(scale_shift), act, _p(out), _dt(out), _row_stride(out), _p(mean), _p(rstd),
-        _p(workspace), workspace.numel() * workspace.element_size(), _stream(x)), what)
+    _gn_check(what, B, n, C_, groups, act)
+    dev, f32 = x.get_device(), torch.float32
+    ldx, ldo = _mat(what, "x", x, B * n, C_, x.dtype, dev), _mat(what, "out", out, B * n, C_, out.dtype, dev)
+    lds = 0 if scale_shift is None else _mat(what, "scale_shift", scale_shift, B, 2 * C_, f32, dev)
+    rc = _lib.load().uwir_group_norm_act(
+        x.data_ptr(), _dt(x), ldx, B, n, C_, groups, eps, _vec(what, "gamma", gamma, (C_,), dev), _vec(what, "beta", beta, (C_,), dev),
+        _p(scale_shift), lds, act, out.data_ptr(), _dt(out), ldo,
+        None if mean is None else _vec(what, "mean", mean, (B, groups), dev),
+        None if rstd is None else _vec(what, "rstd", rstd, (B, groups), dev), workspace.data_ptr(), _scratch(what, workspace, dev),
+        _stream(x))
+    if rc:
+        _lib.check(rc, what)
 
 
 def group_norm_act_backward(dy: torch.Tensor, x: torch.Tensor, B: int, n: int, C_: int, groups: int, gamma: torch.Tensor,
@@ -413,24 +415,23 @@ def group_norm_act_backward(dy: torch.Tensor, x: torch.Tensor, B: int, n: int, C
     """Gradients of ``group_norm_act``: dx [B * n, C] (dtype of x and dy; may be either of them), dgamma, dbeta [C] fp32 and
     dscale_shift [B, 2C] fp32 (written, not added to) from the forward call's x, mean and rstd."""
     what = "group_norm_act_backward"
-    _gn_check(what, x, B, n, C_, groups, gamma, beta, act, scale_shift, workspace)
-    _rows_cols(what, "dy", dy, B * n, C_)
-    _rows_cols(what, "dx", dx, B * n, C_)
-    if dy.dtype != x.dtype or dx.dtype != x.dtype:
-        raise TypeError(f"{what}: x, dy and dx must share a dtype")
-    for name, t, shape in (("mean", mean, (B, groups)), ("rstd", rstd, (B, groups)), ("dgamma", dgamma, (C_,)), ("dbeta", dbeta, (C_,))):
-        _vector(what, name, t, *shape)
+    _gn_check(what, B, n, C_, groups, act)
+    dev, dt, f32, M = x.get_device(), x.dtype, torch.float32, B * n
+    ldy, ldx, ldd = _mat(what, "dy", dy, M, C_, dt, dev), _mat(what, "x", x, M, C_, dt, dev), _mat(what, "dx", dx, M, C_, dt, dev)
+    lds = ldds = 0
+    if scale_shift is not None:
+        lds = _mat(what, "scale_shift", scale_shift, B, 2 * C_, f32, dev)
     if dscale_shift is not None:
         if scale_shift is None:
             raise ValueError(f"{what}: dscale_shift without scale_shift")
-        _f32(dscale_shift)
-        _rows_cols(what, "dscale_shift", dscale_shift, B, 2 * C_)
-    _operands(what, x, dy, gamma, beta, mean, rstd, dx, dgamma, dbeta, workspace, scale_shift, dscale_shift)
-    _lib.check(_lib.load().uwir_group_norm_act_backward(
-        _p(dy), _row_stride(dy), _p(x), _row_stride(x), _dt(x), B, n, C_, groups, _p(gamma), _p(beta), _p(mean), _p(rstd),
-        _p(scale_shift), 0 if scale_shift is None else _row_stride(scale_shift), act, _p(dx), _row_stride(dx), _p(dgamma),
-        _p(dbeta), _p(dscale_shift), 0 if dscale_shift is None else _row_stride(dscale_shift), _p(workspace),
-        workspace.numel() * workspace.element_size(), _stream(x)), what)
+        ldds = _mat(what, "dscale_shift", dscale_shift, B, 2 * C_, f32, dev)
+    rc = _lib.load().uwir_group_norm_act_backward(
+        dy.data_ptr(), ldy, x.data_ptr(), ldx, _dt(x), B, n, C_, groups, _vec(what, "gamma", gamma, (C_,), dev),
+        _vec(what, "beta", beta, (C_,), dev), _vec(what, "mean", mean, (B, groups), dev), _vec(what, "rstd", rstd, (B, groups), dev),
+        _p(scale_shift), lds, act, dx.data_ptr(), ldd, _vec(what, "dgamma", dgamma, (C_,), dev), _vec(what, "dbeta", dbeta, (C_,), dev),
+        _p(dscale_shift), ldds, workspace.data_ptr(), _scratch(what, workspace, dev), _stream(x))
+    if rc:
+        _lib.check(rc, what)
 
 
 def _torch_dt(dtype: torch.dtype) -> int:
@@ -447,25 +448,17 @@ def cross_attn_backward_workspace_bytes(B: int, nq: int, nk: int, heads: int, kv
     return int(_lib.load().uwir_cross_attn_backward_workspace_bytes(B, nq, nk, heads, kv_heads, hd, _torch_dt(dtype)))
 
 
-def _xattn_check(what, q, B, nq, nk, heads, kv_heads, hd, rows, keys, key_lens, key_mask, lse, workspace):
+def _xattn_check(what, B, nq, nk, heads, kv_heads, hd, key_lens, key_mask, workspace, dev) -> tuple:
+    """-> row stride of the mask, bytes of the workspace"""
     if B < 1 or nq < 0 or nk < 0 or heads < 1 or kv_heads < 1 or heads % kv_heads or hd < 1:
         raise ValueError(f"{what}: need B > 0, nq, nk >= 0 and kv_heads dividing heads")
-    for name, t in rows:
-        _rows_cols(what, name, t, B * nq, heads * hd)
-    for name, t in keys:
-        _rows_cols(what, name, t, B * nk, kv_heads * hd)
-    if any(t.dtype != q.dtype for _, t in rows + keys):
-        raise TypeError(f"{what}: {', '.join(n for n, _ in rows + keys)} must share a dtype")
-    if key_lens is not None and (key_lens.dtype != torch.int32 or tuple(key_lens.shape) != (B,) or not key_lens.is_contiguous()):
-        raise ValueError(f"{what}: key_lens must be a contiguous int32 [{B}]")
+    if key_lens is not None and (key_lens.dtype is not torch.int32 or key_lens.shape != (B,) or not key_lens.is_contiguous()
+                                 or key_lens.get_device() != dev):
+        raise ValueError(f"{what}: key_lens must be a contiguous int32 [{B}] with the other operands")
+    ldm = 0
     if key_mask is not None:
-        if key_mask.dtype not in (torch.bool, torch.uint8):
-            raise TypeError(f"{what}: key_mask must be bool or uint8")
-        _rows_cols(what, "key_mask", key_mask, B, nk)
-    _vector(what, "lse", lse, B, heads, nq)
-    if workspace is not None and not workspace.is_contiguous():
-        raise ValueError(f"{what}: workspace must be contiguous")
-    _operands(what, q, *(t for _, t in rows + keys), key_lens, key_mask, lse, workspace)
+        ldm = _mat(what, "key_mask", key_mask, B, nk, torch.uint8 if key_mask.dtype is torch.uint8 else torch.bool, dev)
+    return ldm, (0 if workspace is None else _scratch(what, workspace, dev))
 
 
 def cross_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, B: int, nq: int, nk: int, heads: int, kv_heads: int, hd: int,
@@ -476,12 +469,15 @@ def cross_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, B: int, nq: in
     key_mask[b, index] (bool [B, nk]).  ``lse`` [B, heads, nq] fp32 keeps log sum exp for ``cross_attn_backward``.  An image
     without visible keys gives zeros (lse = -inf).  workspace: cross_attn_workspace_bytes (None if that is 0); see uwir.h."""
     what = "cross_attn"
-    _xattn_check(what, q, B, nq, nk, heads, kv_heads, hd, [("q", q), ("out", out)], [("k", k), ("v", v)], key_lens, key_mask, lse,
-                 workspace)
-    _lib.check(_lib.load().uwir_cross_attn(
-        _p(q), _row_stride(q), _p(k), _row_stride(k), _p(v), _row_stride(v), _dt(q), B, nq, nk, heads, kv_heads, hd, scale,
-        _p(key_lens), _p(key_mask), 0 if key_mask is None else _row_stride(key_mask), _p(out), _row_stride(out), _p(lse),
-        _p(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(), _stream(q)), what)
+    dev, dt, mq, mk, cq, ck = q.get_device(), q.dtype, B * nq, B * nk, heads * hd, kv_heads * hd
+    ldm, nb = _xattn_check(what, B, nq, nk, heads, kv_heads, hd, key_lens, key_mask, workspace, dev)
+    rc = _lib.load().uwir_cross_attn(
+        q.data_ptr(), _mat(what, "q", q, mq, cq, dt, dev), k.data_ptr(), _mat(what, "k", k, mk, ck, dt, dev),
+        v.data_ptr(), _mat(what, "v", v, mk, ck, dt, dev), _dt(q), B, nq, nk, heads, kv_heads, hd, scale, _p(key_lens),
+        _p(key_mask), ldm, out.data_ptr(), _mat(what, "out", out, mq, cq, dt, dev),
+        None if lse is None else _vec(what, "lse", lse, (B, heads, nq), dev), _p(workspace), nb, _stream(q))
+    if rc:
+        _lib.check(rc, what)
 
 
 def cross_attn_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, lse: torch.Tensor, dout: torch.Tensor,
@@ -491,13 +487,17 @@ def cross_attn_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: 
     """Gradients of ``cross_attn`` from its out and lse: dq like q, dk / dv like k / v (written, not added to; zeros at
     invisible keys; summed over the query heads of a shared key head)."""
     what = "cross_attn_backward"
-    _xattn_check(what, q, B, nq, nk, heads, kv_heads, hd, [("q", q), ("out", out), ("dout", dout), ("dq", dq)],
-                 [("k", k), ("v", v), ("dk", dk), ("dv", dv)], key_lens, key_mask, lse, workspace)
-    _lib.check(_lib.load().uwir_cross_attn_backward(
-        _p(q), _row_stride(q), _p(k), _row_stride(k), _p(v), _row_stride(v), _p(out), _row_stride(out), _p(lse), _p(dout),
-        _row_stride(dout), _dt(q), B, nq, nk, heads, kv_heads, hd, scale, _p(key_lens), _p(key_mask),
-        0 if key_mask is None else _row_stride(key_mask), _p(dq), _row_stride(dq), _p(dk), _row_stride(dk), _p(dv),
-        _row_stride(dv), _p(workspace), workspace.numel() * workspace.element_size(), _stream(q)), what)
+    dev, dt, mq, mk, cq, ck = q.get_device(), q.dtype, B * nq, B * nk, heads * hd, kv_heads * hd
+    ldm, nb = _xattn_check(what, B, nq, nk, heads, kv_heads, hd, key_lens, key_mask, workspace, dev)
+    rc = _lib.load().uwir_cross_attn_backward(
+        q.data_ptr(), _mat(what, "q", q, mq, cq, dt, dev), k.data_ptr(), _mat(what, "k", k, mk, ck, dt, dev),
+        v.data_ptr(), _mat(what, "v", v, mk, ck, dt, dev), out.data_ptr(), _mat(what, "out", out, mq, cq, dt, dev),
+        _vec(what, "lse", lse, (B, heads, nq), dev), dout.data_ptr(), _mat(what, "dout", dout, mq, cq, dt, dev), _dt(q),
+        B, nq, nk, heads, kv_heads, hd, scale, _p(key_lens), _p(key_mask), ldm,
+        dq.data_ptr(), _mat(what, "dq", dq, mq, cq, dt, dev), dk.data_ptr(), _mat(what, "dk", dk, mk, ck, dt, dev),
+        dv.data_ptr(), _mat(what, "dv", dv, mk, ck, dt, dev), _p(workspace), nb, _stream(q))
+    if rc:
+        _lib.check(rc, what)
 
 
 def fft_workspace_bytes(B: int, H: int, W: int, C_: int) -> int:
