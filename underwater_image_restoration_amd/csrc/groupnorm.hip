@@ -16,7 +16,8 @@
 namespace {
 
 constexpr int GN_T = 512;          // threads of the streaming kernels
-constexpr int GN_R = 8;            // rows a thread loads ahead of using them
+constexpr int GN_R = 8;            // rows a thread of the resident form holds
+constexpr int GN_RS = 4;           // rows a thread of the streamed form loads ahead of using them
 constexpr int GN_MAX_C = 2048;     // channels of a group, and so of a slab, are bounded by the per-slab sums in LDS
 constexpr int GN_MAX_CHUNKS = 128; // row chunks of an image (each output block sums all partials of its slab)
 
@@ -64,19 +65,19 @@ template <int V> struct Stat {
 #pragma unroll
         for (int j = 0; j < V; ++j) mean[j] = m2[j] = 0.f;
     }
-    // merge `k` <= GN_R fresh rows (pairwise update: exact in the count weights)
-    template <bool FULL, typename T> __device__ __forceinline__ void merge(const Pack<T, V>* p, int k) {
-        const float inv = FULL ? 1.f / GN_R : 1.f / (float)k;
-        const float wa = (float)k / (float)(cnt + k), wb = (float)cnt * wa;
+    // merge `k` <= R fresh rows (pairwise update: exact in the count weights)
+    template <int R, bool FULL, typename T> __device__ __forceinline__ void merge(const Pack<T, V>* p, int k) {
+        const float inv = FULL ? 1.f / R : 1.f / (float)k;
+        const float wa = (float)k * __builtin_amdgcn_rcpf((float)(cnt + k)), wb = (float)cnt * wa;   // weights: an ulp is harmless
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             float s = 0.f;
 #pragma unroll
-            for (int i = 0; i < GN_R; ++i) s += FULL || i < k ? p[i].get(j) : 0.f;
+            for (int i = 0; i < R; ++i) s += FULL || i < k ? p[i].get(j) : 0.f;
             const float m = s * inv;
             float q = 0.f;
 #pragma unroll
-            for (int i = 0; i < GN_R; ++i) {
+            for (int i = 0; i < R; ++i) {
                 const float d = FULL || i < k ? p[i].get(j) - m : 0.f;
                 q = fmaf(d, d, q);
             }
@@ -86,11 +87,31 @@ template <int V> struct Stat {
         }
         cnt += k;
     }
-    template <typename T> __device__ __forceinline__ void batch(const Pack<T, V>* p, int k) {
-        if (k == GN_R) merge<true>(p, k);
-        else if (k > 0) merge<false>(p, k);
+    template <int R, typename T> __device__ __forceinline__ void batch(const Pack<T, V>* p, int k) {
+        if (k == R) merge<R, true>(p, k);
+        else if (k > 0) merge<R, false>(p, k);
+    }
+    // channels of one group put together, `u` neighbours at a time (a power of two): V / u entries remain in front
+    __device__ __forceinline__ void fold(int u) {
+        float half = 0.5f * (float)cnt;
+#pragma unroll
+        for (int w = V; w > 1; w >>= 1)
+            if (u * w > V) {   // another halving
+#pragma unroll
+                for (int j = 0; j < w / 2; ++j) {
+                    const float d = mean[2 * j] - mean[2 * j + 1];
+                    m2[j] = m2[2 * j] + m2[2 * j + 1] + half * d * d;
+                    mean[j] = 0.5f * (mean[2 * j] + mean[2 * j + 1]);
+                }
+                half *= 2.f;
+            }
     }
 };
+
+// neighbouring channels of a thread that always lie in one group
+template <int V> __device__ __forceinline__ int fold_of(int cg) {
+    return cg % V == 0 ? V : (V % cg == 0 ? cg : 1);
+}
 
 // rows r, r + step, ... (k <= R of them; the others repeat row r, which must exist)
 template <int R, typename T, int V>
@@ -109,22 +130,18 @@ __device__ __forceinline__ double shfl_xor_d(double v, int m) {
     return __hiloint2double(__shfl_xor(__double2hiint(v), m), __shfl_xor(__double2loint(v), m));
 }
 
-// Sums of f(g, i), i in [0, m), for every group g of a block, handed to done(g, sum) by one thread each.  Teams of up to a
-// wave; with fewer groups than teams several teams share a group and `scratch` [T / 64 at most] joins them.  Ends with a barrier.
+// For every group g of a block: add(g, lane, lanes, s, q) sums the share of one of `lanes` lanes, done(g, s, q) gets the total
+// in one thread.  Teams of up to a wave; with fewer groups than teams several teams share a group and `scratch` [T / 64] joins
+// them.  Ends with a barrier.
 template <int T, typename F, typename D>
-__device__ __forceinline__ void group_sums(int G, int m, int tid, double2* scratch, F f, D done) {
+__device__ __forceinline__ void group_sums(int G, int tid, double2* scratch, F add, D done) {
     int tpg = 64;
     while (tpg > 1 && tpg * G > T) tpg >>= 1;
     const int teams = T / tpg, lane = tid & (tpg - 1), team = tid / tpg;
     if (G * 2 <= teams) {   // only with whole-wave teams
         const int parts = teams / G, g = team % G, part = team / G;
         double a = 0., b = 0.;
-        if (part < parts)
-            for (int i = part * 64 + lane; i < m; i += parts * 64) {
-                const double2 v = f(g, i);
-                a += v.x;
-                b += v.y;
-            }
+        if (part < parts) add(g, part * 64 + lane, parts * 64, a, b);
         for (int o = 32; o; o >>= 1) {
             a += shfl_xor_d(a, o);
             b += shfl_xor_d(b, o);
@@ -143,12 +160,7 @@ __device__ __forceinline__ void group_sums(int G, int m, int tid, double2* scrat
         for (int g0 = 0; g0 < G; g0 += teams) {   // uniform trip count: the shuffles see whole waves
             const int g = g0 + team;
             double a = 0., b = 0.;
-            if (g < G)
-                for (int i = lane; i < m; i += tpg) {
-                    const double2 v = f(g, i);
-                    a += v.x;
-                    b += v.y;
-                }
+            if (g < G) add(g, lane, tpg, a, b);
             for (int o = tpg >> 1; o; o >>= 1) {
                 a += shfl_xor_d(a, o);
                 b += shfl_xor_d(b, o);
@@ -157,6 +169,20 @@ __device__ __forceinline__ void group_sums(int G, int m, int tid, double2* scrat
         }
     }
     __syncthreads();
+}
+
+// the same over m items a group, item i from f(g, i)
+template <int T, typename F, typename D>
+__device__ __forceinline__ void group_items(int G, int m, int tid, double2* scratch, F f, D done) {
+    group_sums<T>(G, tid, scratch,
+                  [&](int g, int lane, int lanes, double& s, double& q) {
+                      for (int i = lane; i < m; i += lanes) {
+                          const double2 v = f(g, i);
+                          s += v.x;
+                          q += v.y;
+                      }
+                  },
+                  done);
 }
 
 __device__ __forceinline__ float act_silu(float z) { return z * sigmoid_fast(z); }
@@ -174,31 +200,75 @@ struct Place {
         l.ch0 = slab * p.slab;
         l.sc = min(p.slab, p.C - l.ch0);
         l.tw = l.sc / V;
-        l.RL = l.tw <= T ? T / l.tw : 1;
-        l.cv = tid % l.tw;
-        l.rl = tid / l.tw;
+        // quotients of numbers below 2^11 through the reciprocal: (a + 1/2) / b is at least 1 / (2 b) away from an integer
+        const float inv = __builtin_amdgcn_rcpf((float)l.tw);
+        l.RL = l.tw <= T ? (int)((T + 0.5f) * inv) : 1;
+        l.rl = (int)((tid + 0.5f) * inv);
+        l.cv = tid - l.rl * l.tw;
         return l;
     }
 };
 
-// sums of the block's rows per group from the threads' statistics in LDS; `total` rows were dealt to RL row lanes in turn
+// a thread's folded statistics -> LDS, V / fold entries a thread
+template <int V> __device__ __forceinline__ void put_stats(Stat<V>& st, int fold, int tid, float* sm, float* sq) {
+    st.fold(fold);
+    const int e = V / fold;
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+        if (j < e) {
+            sm[tid * e + j] = st.mean[j];
+            sq[tid * e + j] = st.m2[j];
+        }
+    __syncthreads();
+}
+
+// Sums of the block's rows per group from the threads' statistics in LDS: `fold` channels an entry, `total` rows dealt to RL
+// row lanes in turn.  A lane of a group's team keeps to one entry column, or (more columns than lanes) to whole columns.
 template <int T, int V, typename D>
-__device__ __forceinline__ void slab_group_sums(const GnArgs& p, const Place& l, int width, int groups, int total, const float* sm,
-                                                const float* sq, double2* scratch, int tid, D done) {
-    const int cg = p.cg, rows = min(l.RL, max(total, 0)), base = total > 0 ? total / l.RL : 0, rem = total > 0 ? total % l.RL : 0;
-    group_sums<T>(groups, cg * rows, tid, scratch,
-                  [&](int g, int i) {
-                      const int r = i / cg, c = i - r * cg, at = r * width + g * cg + c;
-                      const double k = base + (r < rem), m = sm[at];
-                      return make_double2(k * m, (double)sq[at] + k * m * m);
+__device__ __forceinline__ void slab_group_sums(const GnArgs& p, const Place& l, int fold, int total, const float* sm, const float* sq,
+                                                double2* scratch, int tid, D done) {
+    const int rows = min(l.RL, max(total, 0)), base = total > 0 ? total / l.RL : 0, rem = total > 0 ? total % l.RL : 0;
+    const int width = l.sc / fold, ce = p.cg / fold, groups = l.sc / p.cg;
+    group_sums<T>(groups, tid, scratch,
+                  [&](int g, int lane, int lanes, double& s, double& q) {
+                      const int rl = ce < lanes ? lanes / ce : 1, r0 = ce < lanes ? lane / ce : 0;
+                      if (r0 >= rl) return;
+                      for (int c = ce < lanes ? lane - r0 * ce : lane; c < ce; c += ce < lanes ? ce : lanes)
+                          for (int r = r0; r < rows; r += rl) {
+                              const int at = r * width + g * ce + c;
+                              const double k = (double)((base + (r < rem)) * fold), m = sm[at];
+                              s += k * m;
+                              q += (double)sq[at] + k * m * m;
+                          }
                   },
                   done);
 }
 
 __device__ __forceinline__ float2 finish_stats(double s, double q, double inv_n, float eps) {
     const double m = s * inv_n;
-    const float v = (float)fmax(q * inv_n - m * m, 0.);
+    const float v = fmaxf((float)(q * inv_n - m * m), 0.f);
     return make_float2((float)m, rsqrtf(v + eps));
+}
+
+// V consecutive floats at any alignment of 4 bytes, 16 bytes at a time
+template <int V> __device__ __forceinline__ void load_floats(const float* p, float* o) {
+    if constexpr (V % 4 == 0) {
+#pragma unroll
+        for (int j = 0; j < V; j += 4) __builtin_memcpy(o + j, p + j, 16);
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] = p[j];
+    }
+}
+
+// f(j, g) for the channels c0 + j, j < V, of a slab and the group g each lies in
+template <int V, typename F> __device__ __forceinline__ void each_group(int c0, int cg, F f) {
+    int g = c0 / cg, at = c0 - g * cg;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        f(j, g);
+        if (++at == cg) at = 0, ++g;
+    }
 }
 
 // per-channel coefficients of a thread's V channels: z = (x - m) a + s, xh = (x - m) r; gamma, beta and the modulation are
@@ -206,15 +276,16 @@ __device__ __forceinline__ float2 finish_stats(double s, double q, double inv_n,
 template <int V> struct Coef {
     float w[V], s[V], m[V], r[V];   // w = gamma (1 + scale)
     __device__ __forceinline__ void load(const GnArgs& p, int b, int c0) {
+        load_floats<V>(p.gamma + c0, w);
+        load_floats<V>(p.beta + c0, s);
+        if (p.ss) {
+            float f[V], h[V];
+            load_floats<V>(p.ss + (size_t)b * p.ld_ss + c0, f);
+            load_floats<V>(p.ss + (size_t)b * p.ld_ss + p.C + c0, h);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int c = c0 + j;
-            w[j] = p.gamma[c];
-            s[j] = p.beta[c];
-            if (p.ss) {
-                const float f = 1.f + p.ss[(size_t)b * p.ld_ss + c];
-                w[j] *= f;
-                s[j] = fmaf(s[j], f, p.ss[(size_t)b * p.ld_ss + p.C + c]);
+            for (int j = 0; j < V; ++j) {
+                w[j] *= 1.f + f[j];
+                s[j] = fmaf(s[j], 1.f + f[j], h[j]);
             }
         }
     }
@@ -263,10 +334,10 @@ __global__ void __launch_bounds__(GN_T) gn_stats_kernel(GnArgs p) {
         st.clear();
         if (wide ? cv < l.tw : l.rl < l.RL) {
             const TX* src = X + (size_t)cv * V;
-            row_batches<GN_R>(r0 + (wide ? 0 : l.rl), r1, l.RL, [&](int r, int k) {
-                Pack<TX, V> buf[GN_R];
-                load_rows<GN_R>(buf, src, p.ldx, r, l.RL, k);
-                st.batch(buf, k);
+            row_batches<GN_RS>(r0 + (wide ? 0 : l.rl), r1, l.RL, [&](int r, int k) {
+                Pack<TX, V> buf[GN_RS];
+                load_rows<GN_RS>(buf, src, p.ldx, r, l.RL, k);
+                st.template batch<GN_RS>(buf, k);
             });
         }
         if (wide) {   // a single group: the thread's own sums
@@ -278,20 +349,16 @@ __global__ void __launch_bounds__(GN_T) gn_stats_kernel(GnArgs p) {
             }
             continue;
         }
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            sm[tid * V + j] = st.mean[j];
-            sq[tid * V + j] = st.m2[j];
-        }
-        __syncthreads();
-        slab_group_sums<GN_T, V>(p, l, l.sc, l.sc / p.cg, r1 - r0, sm, sq, scratch, tid,
+        const int fold = fold_of<V>(p.cg);
+        put_stats(st, fold, tid, sm, sq);
+        slab_group_sums<GN_T, V>(p, l, fold, r1 - r0, sm, sq, scratch, tid,
                                  [&](int g, double s, double q) { out[(size_t)g * p.chunks] = make_double2(s, q); });
     }
     if (l.tw > GN_T) {
         double2* all = scratch + GN_T / 64;   // [GN_T], in the place of sm and sq
         all[tid] = make_double2(wide_s, wide_q);
         __syncthreads();
-        group_sums<GN_T>(1, GN_T, tid, scratch, [&](int, int i) { return all[i]; },
+        group_items<GN_T>(1, GN_T, tid, scratch, [&](int, int i) { return all[i]; },
                          [&](int, double s, double q) { out[0] = make_double2(s, q); });
     }
 }
@@ -312,7 +379,7 @@ __global__ void __launch_bounds__(GN_T, 4) gn_apply_kernel(GnArgs p) {
     const bool works = !wide && l.rl < l.RL && r0 + l.rl < r1;
     if (works) co.load(p, b, l.ch0 + l.cv * V);   // on their way while the statistics are put together
     const double2* part = p.part + ((size_t)b * p.G + g0) * p.chunks;
-    group_sums<GN_T>(l.sc / cg, p.chunks, tid, scratch, [&](int g, int i) { return part[(size_t)g * p.chunks + i]; },
+    group_items<GN_T>(l.sc / cg, p.chunks, tid, scratch, [&](int g, int i) { return part[(size_t)g * p.chunks + i]; },
                      [&](int g, double s, double q) {
                          const float2 st = finish_stats(s, q, p.inv_n, p.eps);
                          gst[g] = st;
@@ -322,15 +389,11 @@ __global__ void __launch_bounds__(GN_T, 4) gn_apply_kernel(GnArgs p) {
                          }
                      });
     auto walk = [&](int cv, int r, int step) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const float2 st = gst[wide ? 0 : (cv * V + j) / cg];
-            co.stats(j, st.x, st.y);
-        }
-        row_batches<GN_R / 2>(r, r1, step, [&](int r, int k) {
-            Pack<TX, V> buf[GN_R / 2];
-            load_rows<GN_R / 2>(buf, X + cv * V, p.ldx, r, step, k);
-            emit<GN_R / 2>(buf, co, Y + cv * V, p.ldo, r, step, k, silu);
+        each_group<V>(cv * V, cg, [&](int j, int g) { co.stats(j, gst[g].x, gst[g].y); });
+        row_batches<GN_RS>(r, r1, step, [&](int r, int k) {
+            Pack<TX, V> buf[GN_RS];
+            load_rows<GN_RS>(buf, X + cv * V, p.ldx, r, step, k);
+            emit<GN_RS>(buf, co, Y + cv * V, p.ldo, r, step, k, silu);
         });
     };
     if (works) walk(l.cv, r0 + l.rl, l.RL);
@@ -362,25 +425,17 @@ __global__ void __launch_bounds__(T) gn_resident_kernel(GnArgs p) {
     }
     Stat<V> st;
     st.clear();
-    st.batch(buf, k);
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        sm[tid * V + j] = st.mean[j];
-        sq[tid * V + j] = st.m2[j];
-    }
-    __syncthreads();
-    slab_group_sums<T, V>(p, l, l.sc, l.sc / cg, p.n, sm, sq, scratch, tid, [&](int g, double s, double q) {
+    st.template batch<GN_R>(buf, k);
+    const int fold = fold_of<V>(cg);
+    put_stats(st, fold, tid, sm, sq);
+    slab_group_sums<T, V>(p, l, fold, p.n, sm, sq, scratch, tid, [&](int g, double s, double q) {
         const float2 f = finish_stats(s, q, p.inv_n, p.eps);
         gst[g] = f;
         if (p.mean) p.mean[(size_t)b * p.G + g0 + g] = f.x;
         if (p.rstd) p.rstd[(size_t)b * p.G + g0 + g] = f.y;
     });
     if (k <= 0) return;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const float2 f = gst[(l.cv * V + j) / cg];
-        co.stats(j, f.x, f.y);
-    }
+    each_group<V>(l.cv * V, cg, [&](int j, int g) { co.stats(j, gst[g].x, gst[g].y); });
     emit<GN_R>(buf, co, (TO*)p.out + (size_t)b * p.n * p.ldo + l.ch0 + l.cv * V, p.ldo, l.rl, l.RL, k, p.act == UWIR_ACT_SILU);
 }
 
@@ -390,11 +445,8 @@ __global__ void __launch_bounds__(T) gn_resident_kernel(GnArgs p) {
 template <int V, typename T>
 __device__ __forceinline__ void bwd_stats(const GnArgs& p, Coef<V>& co, int b, int c0) {
     co.load(p, b, c0);
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const int g = (c0 + j) / p.cg;
-        co.stats(j, p.mean_in[(size_t)b * p.G + g], p.rstd_in[(size_t)b * p.G + g]);
-    }
+    const float *m = p.mean_in + (size_t)b * p.G, *r = p.rstd_in + (size_t)b * p.G;
+    each_group<V>(c0, p.cg, [&](int j, int g) { co.stats(j, m[g], r[g]); });
 }
 
 // adds a batch of rows: s1 += sum dz, s2 += sum dz d.  A short chain per batch keeps the fp32 sums close to pairwise.
@@ -571,8 +623,8 @@ __global__ void __launch_bounds__(GN_T, 4) gn_bwd_apply_kernel(GnArgs p) {
         return;
     }
     double2* scratch = reinterpret_cast<double2*>(smem);            // [GN_T / 64]
-    double2* ch = scratch + GN_T / 64;                              // [slab] w (S1, S2)
-    float2* gm = reinterpret_cast<float2*>(ch + p.slab);            // [slab / cg] (m1, m2)
+    double2* ch = scratch + GN_T / 64;                              // [max(slab, GN_T)] sums, then w (S1, S2)
+    float2* gm = reinterpret_cast<float2*>(ch + max(p.slab, GN_T)); // [slab / cg] (m1, m2)
     const Place l = Place::of<V>(p, blockIdx.y, b, tid, GN_T);
     const int cg = p.cg;
     const int r0 = chunk * p.rows, r1 = min(p.n, r0 + p.rows);
@@ -580,33 +632,42 @@ __global__ void __launch_bounds__(GN_T, 4) gn_bwd_apply_kernel(GnArgs p) {
     const T* DY = (const T*)p.dy + (size_t)b * p.n * p.ldy + l.ch0;
     T* DX = (T*)p.out + (size_t)b * p.n * p.ldo + l.ch0;
     const bool silu = p.act == UWIR_ACT_SILU, wide = l.tw > GN_T;
-    for (int c = tid; c < l.sc; c += GN_T) {
+    // the slab's channel sums: lanes of a channel share the chunks, and are joined in LDS (a wide slab has one lane each)
+    const int lanes = l.sc < GN_T ? GN_T / l.sc : 1, cl = l.sc < GN_T ? tid % l.sc : tid, ln = l.sc < GN_T ? tid / l.sc : 0;
+    for (int c = cl; c < l.sc && ln < lanes; c += GN_T) {
         double a = 0., q = 0.;
         const float2* src = p.sums + (size_t)b * p.sum_chunks * p.C + l.ch0 + c;
-#pragma unroll 8
-        for (int i = 0; i < p.sum_chunks; ++i) {
+#pragma unroll 4
+        for (int i = ln; i < p.sum_chunks; i += lanes) {
             const float2 v = src[(size_t)i * p.C];
             a += v.x;
             q += v.y;
         }
-        const int cc = l.ch0 + c;
-        const double w = (double)p.gamma[cc] * (p.ss ? 1. + (double)p.ss[(size_t)b * p.ld_ss + cc] : 1.);
-        ch[c] = make_double2(w * a, w * q);
-        if (chunk == 0) put_dss(p, b, cc, a, q);
+        ch[ln * l.sc + c] = make_double2(a, q);
     }
     __syncthreads();
-    group_sums<GN_T>(l.sc / cg, cg, tid, scratch, [&](int g, int i) { return ch[g * cg + i]; },
+    for (int c = tid; c < l.sc; c += GN_T) {
+        double2 v = ch[c];
+        for (int i = 1; i < lanes; ++i) {
+            v.x += ch[i * l.sc + c].x;
+            v.y += ch[i * l.sc + c].y;
+        }
+        const int cc = l.ch0 + c;
+        const double w = (double)p.gamma[cc] * (p.ss ? 1. + (double)p.ss[(size_t)b * p.ld_ss + cc] : 1.);
+        if (chunk == 0) put_dss(p, b, cc, v.x, v.y);
+        ch[c] = make_double2(w * v.x, w * v.y);
+    }
+    __syncthreads();
+    group_items<GN_T>(l.sc / cg, cg, tid, scratch, [&](int g, int i) { return ch[g * cg + i]; },
                      [&](int g, double s, double q) { gm[g] = make_float2((float)(s * p.inv_n), (float)(q * p.inv_n)); });
     auto walk = [&](int cv, int r, int step) {
         Coef<V> co;
         float u1[V], u2[V];
         bwd_stats<V, T>(p, co, b, l.ch0 + cv * V);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const float2 g = gm[wide ? 0 : (cv * V + j) / cg];
-            u1[j] = co.r[j] * g.x;
-            u2[j] = co.r[j] * co.r[j] * g.y;
-        }
+        each_group<V>(cv * V, cg, [&](int j, int g) {
+            u1[j] = co.r[j] * gm[g].x;
+            u2[j] = co.r[j] * co.r[j] * gm[g].y;
+        });
         row_batches<GN_RB>(r, r1, step, [&](int r, int k) {
             Pack<T, V> bx[GN_RB], bd[GN_RB];
             load_rows<GN_RB>(bx, X + cv * V, p.ldx, r, step, k);
@@ -680,16 +741,14 @@ __global__ void __launch_bounds__(TH) gn_bwd_resident_kernel(GnArgs p) {
         }
     }
     __syncthreads();
-    group_sums<TH>(l.sc / cg, cg, tid, scratch, [&](int g, int i) { return ch[g * cg + i]; },
+    group_items<TH>(l.sc / cg, cg, tid, scratch, [&](int g, int i) { return ch[g * cg + i]; },
                    [&](int g, double s, double q) { gm[g] = make_float2((float)(s * p.inv_n), (float)(q * p.inv_n)); });
     if (k <= 0) return;
     float u1[V], u2[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const float2 g = gm[(l.cv * V + j) / cg];
-        u1[j] = co.r[j] * g.x;
-        u2[j] = co.r[j] * co.r[j] * g.y;
-    }
+    each_group<V>(l.cv * V, cg, [&](int j, int g) {
+        u1[j] = co.r[j] * gm[g].x;
+        u2[j] = co.r[j] * co.r[j] * gm[g].y;
+    });
     bwd_emit<GN_R>(bx, bd, co, u1, u2, (T*)p.out + (size_t)b * p.n * p.ldo + cb, p.ldo, l.rl, l.RL, k, silu);
 }
 
@@ -798,8 +857,8 @@ template <typename T, int V> void launch_bwd(GnArgs p, hipStream_t st) {
         p.sums = p.csum;
         p.sum_chunks = 1;
     }
-    size_t lds = GN_T / 64 * 16 + (size_t)p.slab * 16 + (size_t)(p.slab / p.cg) * 8;
-    if (lds < 8 * 64 * 16) lds = 8 * 64 * 16;
+    // 8 KB of it serve the blocks that form dgamma and dbeta
+    const size_t lds = GN_T / 64 * 16 + (size_t)(p.slab > GN_T ? p.slab : GN_T) * 16 + (size_t)(p.slab / p.cg) * 8;
     hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V>), dim3(p.chunks, slabs, p.B + 1), dim3(GN_T), lds, st, p);
 }
 
