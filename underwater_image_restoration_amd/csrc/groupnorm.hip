@@ -35,7 +35,10 @@ template <typename T, int V> struct Pack {
         if constexpr (V == 1) v = (T)f;
         else v[j] = (T)f;
     }
-    __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<typename VecT<T, V>::type*>(p) = v; }
+    template <bool BYPASS = false> __device__ __forceinline__ void store(T* p) const {
+        if constexpr (BYPASS) __builtin_nontemporal_store(v, reinterpret_cast<typename VecT<T, V>::type*>(p));
+        else *reinterpret_cast<typename VecT<T, V>::type*>(p) = v;
+    }
 };
 
 struct GnArgs {
@@ -297,7 +300,7 @@ template <int V> struct Coef {
     __device__ __forceinline__ float z(int j, float d) const { return fmaf(d, w[j], s[j]); }
 };
 
-template <int R, typename TX, typename TO, int V>
+template <int R, bool BYPASS = false, typename TX, typename TO, int V>
 __device__ __forceinline__ void emit(const Pack<TX, V>* buf, const Coef<V>& co, TO* dst, size_t ld, int r, int step, int k, bool silu) {
 #pragma unroll
     for (int i = 0; i < R; ++i)
@@ -308,7 +311,7 @@ __device__ __forceinline__ void emit(const Pack<TX, V>* buf, const Coef<V>& co, 
                 const float z = co.z(j, buf[i].get(j) - co.m[j]);
                 o.set(j, silu ? act_silu(z) : z);
             }
-            o.store(dst + (size_t)(r + i * step) * ld);
+            o.template store<BYPASS>(dst + (size_t)(r + i * step) * ld);
         }
 }
 
@@ -363,7 +366,7 @@ __global__ void __launch_bounds__(GN_T) gn_stats_kernel(GnArgs p) {
     }
 }
 
-template <typename TX, typename TO, int V>
+template <typename TX, typename TO, int V, bool BYPASS>
 __global__ void __launch_bounds__(GN_T, 4) gn_apply_kernel(GnArgs p) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     double2* scratch = reinterpret_cast<double2*>(smem);               // [GN_T / 64]
@@ -375,9 +378,14 @@ __global__ void __launch_bounds__(GN_T, 4) gn_apply_kernel(GnArgs p) {
     const TX* X = (const TX*)p.x + (size_t)b * p.n * p.ldx + l.ch0;
     TO* Y = (TO*)p.out + (size_t)b * p.n * p.ldo + l.ch0;
     const bool silu = p.act == UWIR_ACT_SILU, wide = l.tw > GN_T;
+    // the first rows and the coefficients are on their way while the statistics are put together
     Coef<V> co;
-    const bool works = !wide && l.rl < l.RL && r0 + l.rl < r1;
-    if (works) co.load(p, b, l.ch0 + l.cv * V);   // on their way while the statistics are put together
+    Pack<TX, V> buf[GN_RS];
+    const int ra = r0 + l.rl, rest = wide || l.rl >= l.RL || ra >= r1 ? 0 : (r1 - ra + l.RL - 1) / l.RL, ka = min(rest, GN_RS);
+    if (rest) {
+        load_rows<GN_RS>(buf, X + l.cv * V, p.ldx, ra, l.RL, ka);
+        co.load(p, b, l.ch0 + l.cv * V);
+    }
     const double2* part = p.part + ((size_t)b * p.G + g0) * p.chunks;
     group_items<GN_T>(l.sc / cg, p.chunks, tid, scratch, [&](int g, int i) { return part[(size_t)g * p.chunks + i]; },
                      [&](int g, double s, double q) {
@@ -388,18 +396,22 @@ __global__ void __launch_bounds__(GN_T, 4) gn_apply_kernel(GnArgs p) {
                              if (p.rstd) p.rstd[(size_t)b * p.G + g0 + g] = st.y;
                          }
                      });
+    auto finish = [&](int cv) { each_group<V>(cv * V, cg, [&](int j, int g) { co.stats(j, gst[g].x, gst[g].y); }); };
     auto walk = [&](int cv, int r, int step) {
-        each_group<V>(cv * V, cg, [&](int j, int g) { co.stats(j, gst[g].x, gst[g].y); });
         row_batches<GN_RS>(r, r1, step, [&](int r, int k) {
-            Pack<TX, V> buf[GN_RS];
             load_rows<GN_RS>(buf, X + cv * V, p.ldx, r, step, k);
-            emit<GN_RS>(buf, co, Y + cv * V, p.ldo, r, step, k, silu);
+            emit<GN_RS, BYPASS>(buf, co, Y + cv * V, p.ldo, r, step, k, silu);
         });
     };
-    if (works) walk(l.cv, r0 + l.rl, l.RL);
+    if (rest) {
+        finish(l.cv);
+        emit<GN_RS, BYPASS>(buf, co, Y + l.cv * V, p.ldo, ra, l.RL, ka, silu);
+        walk(l.cv, ra + GN_RS * l.RL, l.RL);
+    }
     if (wide)
         for (int cv = tid; cv < l.tw; cv += GN_T) {
             co.load(p, b, l.ch0 + cv * V);
+            finish(cv);
             walk(cv, r0, 1);
         }
 }
@@ -471,7 +483,7 @@ __device__ __forceinline__ void bwd_batch(const Pack<T, V>* bx, const Pack<T, V>
 }
 
 // dx = r (w dz - m1 - xh m2) with u1 = r m1, u2 = r^2 m2
-template <int R, typename T, int V>
+template <int R, bool BYPASS = false, typename T, int V>
 __device__ __forceinline__ void bwd_emit(const Pack<T, V>* bx, const Pack<T, V>* bd, const Coef<V>& co, const float* u1, const float* u2,
                                          T* dst, size_t ld, int r, int step, int k, bool silu) {
 #pragma unroll
@@ -485,7 +497,7 @@ __device__ __forceinline__ void bwd_emit(const Pack<T, V>* bx, const Pack<T, V>*
                 if (silu) dz *= dact_silu(co.z(j, d));
                 o.set(j, fmaf(co.w[j], dz, -fmaf(d, u2[j], u1[j])));
             }
-            o.store(dst + (size_t)(r + i * step) * ld);
+            o.template store<BYPASS>(dst + (size_t)(r + i * step) * ld);
         }
 }
 
@@ -611,7 +623,7 @@ __device__ __forceinline__ void put_dss(const GnArgs& p, int b, int c, double s1
 }
 
 // output pass; the last row of blocks (b == B) forms dgamma, dbeta instead
-template <typename T, int V>
+template <typename T, int V, bool BYPASS>
 __global__ void __launch_bounds__(GN_T, 4) gn_bwd_apply_kernel(GnArgs p) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, chunk = blockIdx.x, b = blockIdx.z;
@@ -632,6 +644,15 @@ __global__ void __launch_bounds__(GN_T, 4) gn_bwd_apply_kernel(GnArgs p) {
     const T* DY = (const T*)p.dy + (size_t)b * p.n * p.ldy + l.ch0;
     T* DX = (T*)p.out + (size_t)b * p.n * p.ldo + l.ch0;
     const bool silu = p.act == UWIR_ACT_SILU, wide = l.tw > GN_T;
+    // the first rows and the coefficients are on their way while the sums are put together
+    Coef<V> co;
+    Pack<T, V> bx[GN_RB], bd[GN_RB];
+    const int ra = r0 + l.rl, rest = wide || l.rl >= l.RL || ra >= r1 ? 0 : (r1 - ra + l.RL - 1) / l.RL, ka = min(rest, GN_RB);
+    if (rest) {
+        load_rows<GN_RB>(bx, X + l.cv * V, p.ldx, ra, l.RL, ka);
+        load_rows<GN_RB>(bd, DY + l.cv * V, p.ldy, ra, l.RL, ka);
+        bwd_stats<V, T>(p, co, b, l.ch0 + l.cv * V);
+    }
     // the slab's channel sums: lanes of a channel share the chunks, and are joined in LDS (a wide slab has one lane each)
     const int lanes = l.sc < GN_T ? GN_T / l.sc : 1, cl = l.sc < GN_T ? tid % l.sc : tid, ln = l.sc < GN_T ? tid / l.sc : 0;
     for (int c = cl; c < l.sc && ln < lanes; c += GN_T) {
@@ -660,25 +681,31 @@ __global__ void __launch_bounds__(GN_T, 4) gn_bwd_apply_kernel(GnArgs p) {
     __syncthreads();
     group_items<GN_T>(l.sc / cg, cg, tid, scratch, [&](int g, int i) { return ch[g * cg + i]; },
                      [&](int g, double s, double q) { gm[g] = make_float2((float)(s * p.inv_n), (float)(q * p.inv_n)); });
-    auto walk = [&](int cv, int r, int step) {
-        Coef<V> co;
-        float u1[V], u2[V];
-        bwd_stats<V, T>(p, co, b, l.ch0 + cv * V);
+    float u1[V], u2[V];
+    auto finish = [&](int cv) {
         each_group<V>(cv * V, cg, [&](int j, int g) {
             u1[j] = co.r[j] * gm[g].x;
             u2[j] = co.r[j] * co.r[j] * gm[g].y;
         });
+    };
+    auto walk = [&](int cv, int r, int step) {
         row_batches<GN_RB>(r, r1, step, [&](int r, int k) {
-            Pack<T, V> bx[GN_RB], bd[GN_RB];
             load_rows<GN_RB>(bx, X + cv * V, p.ldx, r, step, k);
             load_rows<GN_RB>(bd, DY + cv * V, p.ldy, r, step, k);
-            bwd_emit<GN_RB>(bx, bd, co, u1, u2, DX + cv * V, p.ldo, r, step, k, silu);
+            bwd_emit<GN_RB, BYPASS>(bx, bd, co, u1, u2, DX + cv * V, p.ldo, r, step, k, silu);
         });
     };
+    if (rest) {
+        finish(l.cv);
+        bwd_emit<GN_RB, BYPASS>(bx, bd, co, u1, u2, DX + l.cv * V, p.ldo, ra, l.RL, ka, silu);
+        walk(l.cv, ra + GN_RB * l.RL, l.RL);
+    }
     if (wide)
-        for (int cv = tid; cv < l.tw; cv += GN_T) walk(cv, r0, 1);
-    else if (l.rl < l.RL)
-        walk(l.cv, r0 + l.rl, l.RL);
+        for (int cv = tid; cv < l.tw; cv += GN_T) {
+            bwd_stats<V, T>(p, co, b, l.ch0 + cv * V);
+            finish(cv);
+            walk(cv, r0, 1);
+        }
 }
 
 template <typename T, int V, int TH>
@@ -775,10 +802,11 @@ int resident_threads(int n, int slab, int cg, int V) {
     return 0;
 }
 
-// row chunks of the streamed form: two blocks per CU over the whole launch, a batch of rows a thread at least.  An upper bound
-// over the slab widths (any vector width), so that the workspace's size does not depend on alignment.
+// row chunks of the streamed form: one block per CU over the whole launch (a block's way through its statistics costs about
+// 3 us whatever its rows: 8 x 64 x 64 x 256 bf16 15.0 us with one, 16.7 with two, 22.9 with four), 16 rows at least.  The
+// workspace counts a single slab: an upper bound that does not depend on vector width, and so not on alignment.
 int stream_chunks(int B, int n, int slabs) {
-    long long c = 512 / ((long long)B * slabs);
+    long long c = 256 / ((long long)B * slabs);
     c = c < 1 ? 1 : (c > GN_MAX_CHUNKS ? GN_MAX_CHUNKS : c);
     const int most = ceil_div(n, 16);
     return c < most ? (int)c : most;
@@ -806,6 +834,10 @@ template <typename F> int with_v(int V, F f) {
     }
 }
 
+// What the second pass reads again was read by the first: where rows in and out together outgrow the memory-side cache (256 MB),
+// written rows would drive out rows still to come, so they go past it (backward over 8 x 256 x 256 x 64 fp32: 117 -> 102 us).
+bool bypass_caches(const GnArgs& p, size_t row_bytes) { return (size_t)p.B * p.n * row_bytes > ((size_t)256 << 20); }
+
 void stream_shape(GnArgs& p, int V, int es) {
     p.slab = slab_channels(p.C, p.cg, V, es, 128);
     p.chunks = stream_chunks(p.B, p.n, ceil_div(p.C, p.slab));
@@ -829,7 +861,11 @@ template <typename TX, typename TO, int V> void launch_fwd(GnArgs p, hipStream_t
     const dim3 grid(p.chunks, ceil_div(p.C, p.slab), p.B);
     const size_t scratch = GN_T / 64 * 16;
     hipLaunchKernelGGL((gn_stats_kernel<TX, V>), grid, dim3(GN_T), scratch + (size_t)GN_T * (V > 2 ? V : 2) * 8, st, p);
-    hipLaunchKernelGGL((gn_apply_kernel<TX, TO, V>), grid, dim3(GN_T), scratch + (size_t)(p.slab / p.cg) * 8, st, p);
+    const size_t lds = scratch + (size_t)(p.slab / p.cg) * 8;
+    if (bypass_caches(p, (size_t)p.C * (sizeof(TX) + sizeof(TO))))
+        hipLaunchKernelGGL((gn_apply_kernel<TX, TO, V, true>), grid, dim3(GN_T), lds, st, p);
+    else
+        hipLaunchKernelGGL((gn_apply_kernel<TX, TO, V, false>), grid, dim3(GN_T), lds, st, p);
 }
 
 template <typename T, int V> void launch_bwd(GnArgs p, hipStream_t st) {
@@ -859,7 +895,11 @@ template <typename T, int V> void launch_bwd(GnArgs p, hipStream_t st) {
     }
     // 8 KB of it serve the blocks that form dgamma and dbeta
     const size_t lds = GN_T / 64 * 16 + (size_t)(p.slab > GN_T ? p.slab : GN_T) * 16 + (size_t)(p.slab / p.cg) * 8;
-    hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V>), dim3(p.chunks, slabs, p.B + 1), dim3(GN_T), lds, st, p);
+    const dim3 grid(p.chunks, slabs, p.B + 1);
+    if (bypass_caches(p, (size_t)p.C * sizeof(T) * 3))
+        hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, true>), grid, dim3(GN_T), lds, st, p);
+    else
+        hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, false>), grid, dim3(GN_T), lds, st, p);
 }
 
 bool overlaps(const void* a, size_t na, const void* b, size_t nb) {
