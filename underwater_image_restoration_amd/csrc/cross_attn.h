@@ -73,6 +73,19 @@ __device__ __forceinline__ void zero16(f32x16& a) {
     for (int r = 0; r < 16; ++r) a[r] = 0.f;
 }
 
+// 0 or -inf per key, as the scores' initial accumulator: hidden keys cost no instructions in the loops.  `bias` holds one float
+// per key of a 32-key block in LDS.
+__device__ __forceinline__ f32x16 bias_rows(const float* bias, int lane) {
+    f32x16 a;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(bias + 8 * u + 4 * (lane >> 5));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) a[4 * u + j] = v[j];
+    }
+    return a;
+}
+
 // v of this lane and of lane ^ 32, in an order that depends on the half: for symmetric uses
 __device__ __forceinline__ float2 both_halves(float v) {
     const unsigned u = __float_as_uint(v);

@@ -69,7 +69,7 @@ template <typename T, int HD> struct Group {
     }
 
     // scores s of 32 keys -> probabilities; the maximum is only moved when it would rise by more than 2^8
-    __device__ __forceinline__ void softmax(f32x16& s, float c, float thr, float* pr) {
+    __device__ __forceinline__ typename M::Prob softmax(const f32x16& s, float c, float thr) {
         float mx = fmaxf(s[0], s[1]);
 #pragma unroll
         for (int r = 2; r < 16; r += 2) mx = fmaxf(fmaxf(mx, s[r]), s[r + 1]);
@@ -85,7 +85,7 @@ template <typename T, int HD> struct Group {
                 for (int r = 0; r < 16; ++r) o[g][r] *= f;
         }
         const float mc = m * c;
-        float l0 = 0.f, l1 = 0.f;
+        float pr[16], l0 = 0.f, l1 = 0.f;   // the sum is that of the unrounded probabilities: lse keeps fp32's accuracy
 #pragma unroll
         for (int r = 0; r < 16; r += 2) {
             pr[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -mc));
@@ -94,14 +94,9 @@ template <typename T, int HD> struct Group {
             l1 += pr[r + 1];
         }
         l += l0 + l1;
+        return M::pack(pr);
     }
 };
-
-__device__ __forceinline__ void hide(f32x16& s, unsigned bits, int lane) {
-    const unsigned b = bits >> (4 * (lane >> 5));
-#pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = (b >> ((r & 3) + 8 * (r >> 2))) & 1u ? s[r] : -INFINITY;
-}
 
 // out and lse of one lane's row, or its part of a split
 template <typename T, int HD>
@@ -164,7 +159,8 @@ __global__ void __launch_bounds__(256) xattn_tile_kernel(XArgs p) {
     static_assert(KT * L::CPR % 256 == 0, "whole chunks per thread");
     __shared__ __attribute__((aligned(16))) T sK[2][KT * L::STR];
     __shared__ __attribute__((aligned(16))) T sV[2][KT * L::STR];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    __shared__ __attribute__((aligned(16))) float sB[2][KT];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const unsigned vid = xcd_order(blockIdx.x, p.nblocks);
     const int qt = vid % p.qtiles, split = (vid / p.qtiles) % p.splits, bk = vid / p.qtiles / p.splits;
     const int b = bk / p.KV, kv = bk % p.KV;
@@ -203,6 +199,7 @@ __global__ void __launch_bounds__(256) xattn_tile_kernel(XArgs p) {
             *reinterpret_cast<typename M::frag*>(&sK[buf][row * L::STR + d]) = rk[i];
             *reinterpret_cast<typename M::frag*>(&sV[buf][row * L::STR + d]) = rv[i];
         }
+        if (tid < KT) sB[buf][tid] = (bits >> tid) & 1 ? 0.f : -INFINITY;
     };
 
     Group<T, HD> gr[QG];
@@ -226,11 +223,10 @@ __global__ void __launch_bounds__(256) xattn_tile_kernel(XArgs p) {
         if (bits && !idle) {
 #pragma unroll
             for (int kb = 0; kb < KT / 32; ++kb) {
-                const unsigned b32 = (unsigned)(bits >> (32 * kb));
-                if (!b32) continue;
+                const f32x16 bias = bias_rows(&sB[buf][32 * kb], lane);
                 f32x16 s[QG];
 #pragma unroll
-                for (int g = 0; g < QG; ++g) zero16(s[g]);
+                for (int g = 0; g < QG; ++g) s[g] = bias;
                 const T* kr = &sK[buf][(32 * kb + (lane & 31)) * L::STR + (lane >> 5) * L::VEC];
 #pragma unroll
                 for (int ks = 0; ks < Group<T, HD>::KS; ++ks) {
@@ -240,12 +236,7 @@ __global__ void __launch_bounds__(256) xattn_tile_kernel(XArgs p) {
                 }
                 typename M::Prob pb[QG];
 #pragma unroll
-                for (int g = 0; g < QG; ++g) {
-                    if (b32 != ~0u) hide(s[g], b32, lane);
-                    float pr[16];
-                    gr[g].softmax(s[g], c, thr, pr);
-                    pb[g] = M::pack(pr);
-                }
+                for (int g = 0; g < QG; ++g) pb[g] = gr[g].softmax(s[g], c, thr);
 #pragma unroll
                 for (int dg = 0; dg < HD / 32; ++dg)
 #pragma unroll
@@ -275,8 +266,9 @@ __global__ void __launch_bounds__(256) xattn_row_kernel(XArgs p) {
     constexpr int TILE = KT * L::STR;
     constexpr int JOIN = 4 * 32 * (HD + 1) * 4, LOOP = 4 * 2 * TILE * (int)sizeof(T);
     __shared__ __attribute__((aligned(16))) char smem[JOIN > LOOP ? JOIN : LOOP];
+    __shared__ __attribute__((aligned(16))) float sB[4][32];
     __shared__ float sm[4][32], sl[4][32];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     T* sK = reinterpret_cast<T*>(smem) + wave * 2 * TILE;
     T* sV = sK + TILE;
     const unsigned vid = xcd_order(blockIdx.x, p.nblocks);
@@ -322,22 +314,19 @@ __global__ void __launch_bounds__(256) xattn_row_kernel(XArgs p) {
             *reinterpret_cast<typename M::frag*>(sK + row * L::STR + d) = rk[i];
             *reinterpret_cast<typename M::frag*>(sV + row * L::STR + d) = rv[i];
         }
+        if (lane < 32) sB[wave][lane] = (bits >> lane) & 1 ? 0.f : -INFINITY;
         // the wave's own LDS operations stay in order; only the compiler has to be held
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         if (k0 + 4 * KT < end) load(k0 + 4 * KT);
         if (bits) {
-            f32x16 s;
-            zero16(s);
+            f32x16 s = bias_rows(sB[wave], lane);
             const T* kr = sK + (lane & 31) * L::STR + (lane >> 5) * L::VEC;
 #pragma unroll
             for (int ks = 0; ks < Group<T, HD>::KS; ++ks)
                 M::rows(s, *reinterpret_cast<const typename M::frag*>(kr + ks * M::KSTEP), gr.q[ks]);
-            if (bits != ~0u) hide(s, bits, lane);
-            float pr[16];
-            gr.softmax(s, c, thr, pr);
-            const typename M::Prob pb = M::pack(pr);
+            const typename M::Prob pb = gr.softmax(s, c, thr);
 #pragma unroll
             for (int dg = 0; dg < HD / 32; ++dg) M::template cols<L::STR>(gr.o[dg], sV + 32 * dg, lane, pb);
         }
