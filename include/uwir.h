@@ -290,7 +290,7 @@ int uwir_group_norm_act_backward(const void* dy, size_t ldy, const void* x, size
  * the forward call and dout; the gradients of shared key heads are summed over their query heads in a fixed order.
  * All tensors of a call share a dtype (fp32: exact-fp32 MFMA; bf16: bf16 MFMA operands with probabilities and score
  * gradients rounded to bf16, fp32 accumulation and statistics).  hd % 8 == 0, hd <= 128; rows and strides 16-byte aligned;
- * scale > 0; nq, nk >= 0; B * kv_heads <= 65535.  Outputs must not overlap any other operand.
+ * 1e-20 <= scale <= 1e20; row strides below 32 MB; nq, nk >= 0; B * kv_heads <= 65535.  Outputs must not overlap any other operand.
  * workspace: >= the matching *_workspace_bytes (may be 0), 16-byte aligned; calls that may run at the same
  * time need one each (captured graphs included).  Results do not depend on scheduling. */
 size_t uwir_cross_attn_workspace_bytes(int B, int nq, int nk, int heads, int kv_heads, int hd, int dtype);

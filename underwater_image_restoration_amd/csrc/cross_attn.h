@@ -32,17 +32,41 @@ template <> struct Mma<bf16_t> {
             for (int j = 0; j < 8; ++j) o.p[s][j] = (bf16_t)v[8 * s + j];
         return o;
     }
+    // Hides keys: one more step of rows() in which a hidden key's row carries the type's lowest value and every query a one, so
+    // that its score is about -3.4e38 and its probability 0.  No select per score, no branch, one MFMA of a dozen.
+    static __device__ __forceinline__ frag hider(bool hidden, int lane) {
+        frag f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = (bf16_t)0.f;
+        f[0] = lane < 32 && hidden ? __builtin_bit_cast(bf16_t, (unsigned short)0xff7f) : (bf16_t)0.f;
+        return f;
+    }
+    static __device__ __forceinline__ void hide(f32x16& acc, frag hider, int lane) {
+        frag one;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) one[j] = (bf16_t)(j == 0 ? 1.f : 0.f);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hider, one, acc, 0, 0, 0);
+    }
     // acc[col0 + ., .] += tile[row0 .. row0 + 31][col0 + .]^T * prob.  Lane group of 16: four rows x 16 columns a read.
-    template <int STR> static __device__ __forceinline__ void cols(f32x16& acc, const bf16_t* tile, int lane, const Prob& b) {
+    struct ColFrags { frag f[2]; };
+    template <int STR> static __device__ __forceinline__ ColFrags col_frags(const bf16_t* tile, int lane) {
         typedef __attribute__((address_space(3))) bf16x4 lds4;
         const bf16_t* p = tile + (4 * (lane >> 5) + ((lane & 15) >> 2)) * STR + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+        ColFrags c;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4*)(p + 16 * s * STR));
             const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4*)(p + (16 * s + 8) * STR));
-            acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), b.p[s], acc,
-                                                          0, 0, 0);
+            c.f[s] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         }
+        return c;
+    }
+    static __device__ __forceinline__ void cols(f32x16& acc, const ColFrags& a, const Prob& b) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.f[s], b.p[s], acc, 0, 0, 0);
+    }
+    template <int STR> static __device__ __forceinline__ void cols(f32x16& acc, const bf16_t* tile, int lane, const Prob& b) {
+        cols(acc, col_frags<STR>(tile, lane), b);
     }
 };
 
@@ -60,11 +84,24 @@ template <> struct Mma<float> {
         for (int r = 0; r < 16; ++r) o.p[r] = v[r];
         return o;
     }
-    template <int STR> static __device__ __forceinline__ void cols(f32x16& acc, const float* tile, int lane, const Prob& b) {
+    static __device__ __forceinline__ float hider(bool hidden, int lane) { return lane < 32 && hidden ? -3.38e38f : 0.f; }
+    static __device__ __forceinline__ void hide(f32x16& acc, float hider, int lane) {
+        acc = __builtin_amdgcn_mfma_f32_32x32x2f32(hider, 1.f, acc, 0, 0, 0);
+    }
+    struct ColFrags { float f[16]; };
+    template <int STR> static __device__ __forceinline__ ColFrags col_frags(const float* tile, int lane) {
         const float* p = tile + 4 * (lane >> 5) * STR + (lane & 31);
+        ColFrags c;
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-            acc = __builtin_amdgcn_mfma_f32_32x32x2f32(p[((r & 3) + 8 * (r >> 2)) * STR], b.p[r], acc, 0, 0, 0);
+        for (int r = 0; r < 16; ++r) c.f[r] = p[((r & 3) + 8 * (r >> 2)) * STR];
+        return c;
+    }
+    static __device__ __forceinline__ void cols(f32x16& acc, const ColFrags& a, const Prob& b) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.f[r], b.p[r], acc, 0, 0, 0);
+    }
+    template <int STR> static __device__ __forceinline__ void cols(f32x16& acc, const float* tile, int lane, const Prob& b) {
+        cols(acc, col_frags<STR>(tile, lane), b);
     }
 };
 
@@ -73,17 +110,19 @@ __device__ __forceinline__ void zero16(f32x16& a) {
     for (int r = 0; r < 16; ++r) a[r] = 0.f;
 }
 
-// 0 or -inf per key, as the scores' initial accumulator: hidden keys cost no instructions in the loops.  `bias` holds one float
-// per key of a 32-key block in LDS.
-__device__ __forceinline__ f32x16 bias_rows(const float* bias, int lane) {
-    f32x16 a;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-        const f32x4 v = *reinterpret_cast<const f32x4*>(bias + 8 * u + 4 * (lane >> 5));
-#pragma unroll
-        for (int j = 0; j < 4; ++j) a[4 * u + j] = v[j];
-    }
-    return a;
+// A tile of rows of a matrix in global memory as a buffer: rows from `row` on, of which those below `end` exist; anything
+// beyond reads as zeros, so that neither clamps nor selects sit in the loops.  `ldb`, `width` in bytes, ldb < 2^25.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_buffer(const void* base, size_t ldb, int row, int end, int width) {
+    const size_t bytes = row < end ? (size_t)(end - row - 1) * ldb + width : 0;
+    return __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)base + (size_t)row * ldb), 0,
+                                             (int)(bytes < 0x7fffffff ? bytes : 0x7fffffff), 0x00020000);
+}
+// byte offset of a 16-byte chunk in such a buffer; columns behind the matrix lie behind every buffer
+__device__ __forceinline__ unsigned tile_offset(int row, unsigned ldb, int col_bytes, int width) {
+    return col_bytes < width ? row * ldb + col_bytes : 0x80000000u;
+}
+template <typename F> __device__ __forceinline__ F buffer_frag(__amdgpu_buffer_rsrc_t r, unsigned off) {
+    return __builtin_bit_cast(F, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, 0));
 }
 
 // v of this lane and of lane ^ 32, in an order that depends on the half: for symmetric uses
@@ -147,7 +186,7 @@ inline int xattn_check(const char* what, int dtype, int B, int nq, int nk, int h
     UWIR_CHECK((long long)B * kv_heads <= 65535 && (long long)nq * (heads / kv_heads) < (1ll << 30) && nk < (1 << 30),
                "%s: too large (B * kv_heads <= 65535; nq * heads / kv_heads and nk below 2^30)", what);
     UWIR_CHECK(hd > 0 && hd <= 128 && hd % 8 == 0, "%s: head size must be a multiple of 8, at most 128", what);
-    UWIR_CHECK(scale > 0.f && scale < 1e30f, "%s: scale must be positive and finite", what);
+    UWIR_CHECK(scale >= 1e-20f && scale <= 1e20f, "%s: scale must lie in [1e-20, 1e20]", what);
     return UWIR_OK;
 }
 
@@ -159,6 +198,7 @@ inline int xattn_check_mats(const char* what, int dtype, int hd, const XMat* in,
         if (m.rows == 0) continue;
         UWIR_CHECK(m.p, "%s: null pointer (%s)", what, m.name);
         UWIR_CHECK(m.ld >= (size_t)m.heads * hd, "%s: row stride of %s is below heads * hd", what, m.name);
+        UWIR_CHECK(m.ld * es < (1u << 25), "%s: row stride of %s is 32 MB or more", what, m.name);
         UWIR_CHECK(((uintptr_t)m.p & 15) == 0 && (m.ld * es) % 16 == 0, "%s: rows of %s must be 16-byte aligned", what, m.name);
     }
     // an output may share a wider matrix with another operand (column ranges that do not meet), but no element

@@ -4,7 +4,7 @@
 // image and key head), so shared heads read their keys once.  S^T = K q^T puts a query row on a lane and its keys on the
 // accumulator's registers: maximum and sum are register reductions plus one exchange between the wave's halves, and
 // P feeds O^T += V^T P from registers (cross_attn.h).
-//   tile kernel   4 waves x 32 QG rows share key tiles of 64 in LDS (double buffered, next tile loading meanwhile)
+//   tile kernel   4 waves x 32 QG rows share key tiles in LDS
 //   row kernel    R <= 32: the 4 waves take key tiles of their own and join at the end
 // Either may split the key axis over blocks when there are few rows; a second launch joins the parts.
 #include "cross_attn.h"
@@ -68,24 +68,29 @@ template <typename T, int HD> struct Group {
         l = 0.f;
     }
 
-    // scores s of 32 keys -> probabilities; the maximum is only moved when it would rise by more than 2^8
-    __device__ __forceinline__ typename M::Prob softmax(const f32x16& s, float c, float thr) {
+    // Scores s of 32 keys -> probabilities relative to the running reference m.  m need not be the maximum, only near enough for
+    // the fp32 range: the probabilities are formed first, and only where a lane's sum leaves 2^64 is the true maximum taken, the
+    // output rescaled and the unit formed again (the very first unit does so by itself: m starts at -1e30).  A reference below the
+    // maximum costs no accuracy; what underflows next to it is below 2^-120 of a sum that is at least 1.
+    static __device__ __forceinline__ bool out_of_range(float sum) { return sum > 1.8446744e19f; }
+    __device__ __forceinline__ void rescale(const f32x16& s, float c, typename M::Prob& pb, float& sum) {
         float mx = fmaxf(s[0], s[1]);
 #pragma unroll
         for (int r = 2; r < 16; r += 2) mx = fmaxf(fmaxf(mx, s[r]), s[r + 1]);
         const float2 h = both_halves(mx);
-        mx = fmaxf(h.x, h.y);
-        if (__any(mx > m + thr)) {
-            const float mn = fmaxf(m, mx), f = __builtin_amdgcn_exp2f((m - mn) * c);
-            m = mn;
-            l *= f;
+        const float mn = fmaxf(m, fmaxf(h.x, h.y)), f = __builtin_amdgcn_exp2f((m - mn) * c);
+        m = mn;
+        l *= f;
 #pragma unroll
-            for (int g = 0; g < DG; ++g)
+        for (int g = 0; g < DG; ++g)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) o[g][r] *= f;
-        }
+            for (int r = 0; r < 16; ++r) o[g][r] *= f;
+        pb = form(s, c, sum);
+    }
+    // the sum is that of the unrounded probabilities: lse keeps fp32's accuracy
+    __device__ __forceinline__ typename M::Prob form(const f32x16& s, float c, float& sum) const {
         const float mc = m * c;
-        float pr[16], l0 = 0.f, l1 = 0.f;   // the sum is that of the unrounded probabilities: lse keeps fp32's accuracy
+        float pr[16], l0 = 0.f, l1 = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; r += 2) {
             pr[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -mc));
@@ -93,7 +98,7 @@ template <typename T, int HD> struct Group {
             l0 += pr[r];
             l1 += pr[r + 1];
         }
-        l += l0 + l1;
+        sum = l0 + l1;
         return M::pack(pr);
     }
 };
@@ -102,7 +107,7 @@ template <typename T, int HD> struct Group {
 template <typename T, int HD>
 __device__ __forceinline__ void write_row(const XArgs& p, int b, int kv, int split, int r, int lane, const f32x16* o, float l, float m) {
     if (r >= p.R) return;
-    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const float inv = l > 0.f ? __builtin_amdgcn_rcpf(l) : 0.f;   // 1 ulp
     const float l2 = l > 0.f ? fmaf(m, p.c, __builtin_amdgcn_logf(l)) : -INFINITY;   // v_log_f32: base 2
     const RowRef f = row_ref(p, b, kv, r);
     if (p.splits > 1) {
@@ -151,15 +156,18 @@ __device__ __forceinline__ void key_range(const XArgs& p, int b, int split, int 
     end = min(len, (split + 1) * per * unit);
 }
 
-template <typename T, int HD, int QG>
-__global__ void __launch_bounds__(256) xattn_tile_kernel(XArgs p) {
+// NW waves x 32 QG rows share key tiles of KT keys in LDS (two buffers, the next tile loading meanwhile).  Nothing in a wave's way
+// through a tile overlaps its matrix and its vector work (scores, probabilities, output); the waves of a SIMD do.  With two row groups a wave reads every
+// fragment of K and V from LDS once for both: LDS, not arithmetic, held the one-group form back.
+template <typename T, int HD, int NW, int QG>
+__global__ void __launch_bounds__(NW * 64, QG == 2 ? 2 : 1) xattn_tile_kernel(XArgs p) {
     typedef Tile<T, HD> L;
     typedef typename L::M M;
-    constexpr int KT = 64, NC = KT * L::CPR / 256;   // 16-byte chunks of K (and of V) per thread and tile
-    static_assert(KT * L::CPR % 256 == 0, "whole chunks per thread");
+    typedef typename M::frag frag;
+    constexpr int TH = NW * 64, KT = 64, NC = KT * L::CPR / TH < 1 ? 1 : KT * L::CPR / TH;   // 16-byte chunks per thread and tile
+    static_assert(KT * L::CPR % TH == 0 || KT * L::CPR < TH, "whole chunks per thread");
     __shared__ __attribute__((aligned(16))) T sK[2][KT * L::STR];
     __shared__ __attribute__((aligned(16))) T sV[2][KT * L::STR];
-    __shared__ __attribute__((aligned(16))) float sB[2][KT];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const unsigned vid = xcd_order(blockIdx.x, p.nblocks);
     const int qt = vid % p.qtiles, split = (vid / p.qtiles) % p.splits, bk = vid / p.qtiles / p.splits;
@@ -170,44 +178,47 @@ __global__ void __launch_bounds__(256) xattn_tile_kernel(XArgs p) {
     const T* K = (const T*)p.k + (size_t)b * p.nk * p.ldk + (size_t)kv * p.hd;
     const T* V = (const T*)p.v + (size_t)b * p.nk * p.ldv + (size_t)kv * p.hd;
     const unsigned char* mask = p.mask ? p.mask + (size_t)b * p.ldm : nullptr;
-
-    typename M::frag rk[NC], rv[NC];
+    const int width = p.hd * (int)sizeof(T);
+    const size_t ldkb = p.ldk * sizeof(T), ldvb = p.ldv * sizeof(T);
+    const bool loads = KT * L::CPR >= TH || tid < KT * L::CPR;
+    unsigned ko[NC], vo[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        const int row = (tid + TH * i) / L::CPR, col = (tid + TH * i) % L::CPR * 16;
+        ko[i] = tile_offset(row, (unsigned)ldkb, col, width);
+        vo[i] = tile_offset(row, (unsigned)ldvb, col, width);
+    }
+    frag rk[NC], rv[NC];
     bool vis;
     auto load = [&](int k0) {
+        const __amdgpu_buffer_rsrc_t kr = tile_buffer(K, ldkb, k0, end, width), vr = tile_buffer(V, ldvb, k0, end, width);
+        if (loads) {
 #pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            const int ci = tid + 256 * i, d = (ci % L::CPR) * L::VEC, key = min(k0 + ci / L::CPR, end - 1);
-            if (d < p.hd) {
-                rk[i] = *reinterpret_cast<const typename M::frag*>(K + (size_t)key * p.ldk + d);
-                rv[i] = *reinterpret_cast<const typename M::frag*>(V + (size_t)key * p.ldv + d);
-            } else {
-#pragma unroll
-                for (int j = 0; j < L::VEC; ++j) rk[i][j] = rv[i][j] = (T)0.f;
+            for (int i = 0; i < NC; ++i) {
+                rk[i] = buffer_frag<frag>(kr, ko[i]);
+                rv[i] = buffer_frag<frag>(vr, vo[i]);
             }
         }
         vis = k0 + lane < end && (!mask || mask[k0 + lane]);
     };
-    // hidden keys enter as zeros: what they hold (NaN included) must not meet the zero probabilities
+    // keys hidden by the mask enter as zeros: what they hold (NaN included) must not meet the zero probabilities
     auto store = [&](int buf, unsigned long long bits) {
+        if (!loads) return;
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
-            const int ci = tid + 256 * i, row = ci / L::CPR, d = (ci % L::CPR) * L::VEC;
-            if (bits != ~0ull && !((bits >> row) & 1)) {
-#pragma unroll
-                for (int j = 0; j < L::VEC; ++j) rk[i][j] = rv[i][j] = (T)0.f;
-            }
-            *reinterpret_cast<typename M::frag*>(&sK[buf][row * L::STR + d]) = rk[i];
-            *reinterpret_cast<typename M::frag*>(&sV[buf][row * L::STR + d]) = rv[i];
+            const int row = (tid + TH * i) / L::CPR, d = (tid + TH * i) % L::CPR * L::VEC;
+            if (mask && !((bits >> row) & 1)) rk[i] = rv[i] = frag{};
+            *reinterpret_cast<frag*>(&sK[buf][row * L::STR + d]) = rk[i];
+            *reinterpret_cast<frag*>(&sV[buf][row * L::STR + d]) = rv[i];
         }
-        if (tid < KT) sB[buf][tid] = (bits >> tid) & 1 ? 0.f : -INFINITY;
     };
 
     Group<T, HD> gr[QG];
-    const int row0 = (qt * 4 + wave) * 32 * QG + (lane & 31);
+    const int first = (qt * NW + wave) * 32 * QG, row0 = first + (lane & 31);
 #pragma unroll
     for (int g = 0; g < QG; ++g) gr[g].init(p, b, kv, row0 + 32 * g, lane);
-    const float c = p.c, thr = 8.f / c;
-    const bool idle = (qt * 4 + wave) * 32 * QG >= p.R;   // the whole wave lies behind the last row
+    const float c = p.c;
+    const bool idle = first >= p.R;   // the whole wave lies behind the last row: it only helps to load
 
     unsigned long long bits = 0;
     if (begin < end) {
@@ -223,25 +234,38 @@ __global__ void __launch_bounds__(256) xattn_tile_kernel(XArgs p) {
         if (bits && !idle) {
 #pragma unroll
             for (int kb = 0; kb < KT / 32; ++kb) {
-                const f32x16 bias = bias_rows(&sB[buf][32 * kb], lane);
                 f32x16 s[QG];
 #pragma unroll
-                for (int g = 0; g < QG; ++g) s[g] = bias;
+                for (int g = 0; g < QG; ++g) zero16(s[g]);
                 const T* kr = &sK[buf][(32 * kb + (lane & 31)) * L::STR + (lane >> 5) * L::VEC];
 #pragma unroll
                 for (int ks = 0; ks < Group<T, HD>::KS; ++ks) {
-                    const typename M::frag kf = *reinterpret_cast<const typename M::frag*>(kr + ks * M::KSTEP);
+                    const frag kf = *reinterpret_cast<const frag*>(kr + ks * M::KSTEP);
 #pragma unroll
                     for (int g = 0; g < QG; ++g) M::rows(s[g], kf, gr[g].q[ks]);
                 }
+                const auto hider = M::hider(!(((unsigned)(bits >> (32 * kb)) >> (lane & 31)) & 1), lane);
+#pragma unroll
+                for (int g = 0; g < QG; ++g) M::hide(s[g], hider, lane);
                 typename M::Prob pb[QG];
+                float sum[QG];
+                bool far = false;
 #pragma unroll
-                for (int g = 0; g < QG; ++g) pb[g] = gr[g].softmax(s[g], c, thr);
+                for (int g = 0; g < QG; ++g) {
+                    pb[g] = gr[g].form(s[g], c, sum[g]);
+                    far |= gr[g].out_of_range(sum[g]);
+                }
+                if (__any(far))
 #pragma unroll
-                for (int dg = 0; dg < HD / 32; ++dg)
+                    for (int g = 0; g < QG; ++g) gr[g].rescale(s[g], c, pb[g], sum[g]);
 #pragma unroll
-                    for (int g = 0; g < QG; ++g)
-                        M::template cols<L::STR>(gr[g].o[dg], &sV[buf][32 * kb * L::STR + 32 * dg], lane, pb[g]);
+                for (int g = 0; g < QG; ++g) gr[g].l += sum[g];
+#pragma unroll
+                for (int dg = 0; dg < HD / 32; ++dg) {
+                    const auto vf = M::template col_frags<L::STR>(&sV[buf][32 * kb * L::STR + 32 * dg], lane);
+#pragma unroll
+                    for (int g = 0; g < QG; ++g) M::cols(gr[g].o[dg], vf, pb[g]);
+                }
             }
         }
         if (more) {
@@ -266,7 +290,6 @@ __global__ void __launch_bounds__(256) xattn_row_kernel(XArgs p) {
     constexpr int TILE = KT * L::STR;
     constexpr int JOIN = 4 * 32 * (HD + 1) * 4, LOOP = 4 * 2 * TILE * (int)sizeof(T);
     __shared__ __attribute__((aligned(16))) char smem[JOIN > LOOP ? JOIN : LOOP];
-    __shared__ __attribute__((aligned(16))) float sB[4][32];
     __shared__ float sm[4][32], sl[4][32];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     T* sK = reinterpret_cast<T*>(smem) + wave * 2 * TILE;
@@ -299,7 +322,7 @@ __global__ void __launch_bounds__(256) xattn_row_kernel(XArgs p) {
 
     Group<T, HD> gr;
     gr.init(p, b, kv, lane & 31, lane);
-    const float c = p.c, thr = 8.f / c;
+    const float c = p.c;
     int k0 = begin + wave * KT;
     if (k0 < end) load(k0);
     for (; k0 < end; k0 += 4 * KT) {
@@ -314,19 +337,23 @@ __global__ void __launch_bounds__(256) xattn_row_kernel(XArgs p) {
             *reinterpret_cast<typename M::frag*>(sK + row * L::STR + d) = rk[i];
             *reinterpret_cast<typename M::frag*>(sV + row * L::STR + d) = rv[i];
         }
-        if (lane < 32) sB[wave][lane] = (bits >> lane) & 1 ? 0.f : -INFINITY;
         // the wave's own LDS operations stay in order; only the compiler has to be held
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         if (k0 + 4 * KT < end) load(k0 + 4 * KT);
         if (bits) {
-            f32x16 s = bias_rows(sB[wave], lane);
+            f32x16 s;
+            zero16(s);
             const T* kr = sK + (lane & 31) * L::STR + (lane >> 5) * L::VEC;
 #pragma unroll
             for (int ks = 0; ks < Group<T, HD>::KS; ++ks)
                 M::rows(s, *reinterpret_cast<const typename M::frag*>(kr + ks * M::KSTEP), gr.q[ks]);
-            const typename M::Prob pb = gr.softmax(s, c, thr);
+            M::hide(s, M::hider(!((bits >> (lane & 31)) & 1), lane), lane);
+            float sum;
+            typename M::Prob pb = gr.form(s, c, sum);
+            if (__any(gr.out_of_range(sum))) gr.rescale(s, c, pb, sum);
+            gr.l += sum;
 #pragma unroll
             for (int dg = 0; dg < HD / 32; ++dg) M::template cols<L::STR>(gr.o[dg], sV + 32 * dg, lane, pb);
         }
@@ -406,7 +433,8 @@ __global__ void __launch_bounds__(256) xattn_join_kernel(XArgs p) {
 // ---------------------------------------------------------------------------------------- launch rules
 struct Plan {
     bool row;       // row kernel
-    int qg, qtiles, splits;
+    bool two;       // two row groups a wave
+    int qtiles, splits;
 };
 
 int hd_class(int hd) { return hd <= 32 ? 32 : hd <= 64 ? 64 : 128; }
@@ -415,18 +443,18 @@ Plan plan_fwd(int B, int nq, int nk, int H, int KV, int hd, int dtype) {
     Plan pl = {};
     const long long R = (long long)nq * (H / KV), bk = (long long)B * KV;
     pl.row = R <= 32;
-    pl.qg = 1;
+    pl.two = false;
     long long blocks;
-    int unit;   // smallest part worth a block of its own
+    const int unit = 256;   // smallest part worth a block of its own
     if (pl.row) {
         pl.qtiles = 1;
         blocks = bk;
-        unit = 256;
     } else {
-        pl.qg = dtype == UWIR_BF16 && hd <= 64 && R > 128 && (R + 255) / 256 * bk >= 512 ? 2 : 1;
-        pl.qtiles = (int)((R + 128 * pl.qg - 1) / (128 * pl.qg));
+        // where 256 rows a block still give every CU two blocks (bf16; the registers of 128 columns leave no room)
+        pl.two = dtype == UWIR_BF16 && hd <= 64 && R > 128 && (R + 255) / 256 * bk >= 512;
+        const int rows = pl.two ? 256 : 128;
+        pl.qtiles = (int)((R + rows - 1) / rows);
         blocks = bk * pl.qtiles;
-        unit = 256;
     }
     // few blocks: parts of the key axis until every CU has two blocks
     long long s = blocks >= 384 ? 1 : (512 + blocks - 1) / (blocks > 0 ? blocks : 1);
@@ -440,11 +468,11 @@ Plan plan_fwd(int B, int nq, int nk, int H, int KV, int hd, int dtype) {
 template <typename T, int HD> void launch(const XArgs& p, const Plan& pl, hipStream_t st) {
     if (pl.row)
         hipLaunchKernelGGL((xattn_row_kernel<T, HD>), dim3(p.nblocks), dim3(256), 0, st, p);
-    else if (pl.qg == 2) {
+    else if (pl.two) {
         if constexpr (sizeof(T) == 2 && HD <= 64)
-            hipLaunchKernelGGL((xattn_tile_kernel<T, HD, 2>), dim3(p.nblocks), dim3(256), 0, st, p);
+            hipLaunchKernelGGL((xattn_tile_kernel<T, HD, 4, 2>), dim3(p.nblocks), dim3(256), 0, st, p);
     } else
-        hipLaunchKernelGGL((xattn_tile_kernel<T, HD, 1>), dim3(p.nblocks), dim3(256), 0, st, p);
+        hipLaunchKernelGGL((xattn_tile_kernel<T, HD, 4, 1>), dim3(p.nblocks), dim3(256), 0, st, p);
     if (p.splits > 1) {
         const size_t n = (size_t)p.B * p.KV * p.R * (p.hd / 8);
         hipLaunchKernelGGL((xattn_join_kernel<T>), dim3((unsigned)ceil_div_sz(n, 256)), dim3(256), 0, st, p);
