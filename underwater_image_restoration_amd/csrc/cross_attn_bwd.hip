@@ -64,8 +64,9 @@ __global__ void __launch_bounds__(256) xattn_dq_kernel(BArgs p) {
     __shared__ __attribute__((aligned(16))) T sV[2][KT * L::STR];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const unsigned vid = xcd_order(blockIdx.x, p.qblocks);
-    const int qt = vid % p.qtiles, split = (vid / p.qtiles) % p.qsplits, bk = vid / p.qtiles / p.qsplits;
-    const int b = bk / p.KV, kv = bk % p.KV;
+    // heads next to each other: the blocks that run together then read whole rows (cross_attn.hip)
+    const int kv = vid % p.KV, qt = vid / p.KV % p.qtiles, bs = vid / p.KV / p.qtiles, split = bs % p.qsplits, b = bs / p.qsplits;
+    const int bk = b * p.KV + kv;
     int begin = 0, end = image_len(p, b);
     if (p.qsplits > 1) {
         const int tiles = (end + KT - 1) / KT, per = (tiles + p.qsplits - 1) / p.qsplits;
@@ -234,8 +235,8 @@ __global__ void __launch_bounds__(256) xattn_dkv_kernel(BArgs p) {
     T* sG = sQ + 2 * TILE;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, kw = wave % KW, wr = wave / KW;
     const unsigned vid = xcd_order(blockIdx.x, p.kblocks);
-    const int kt = vid % p.ktiles, split = (vid / p.ktiles) % p.ksplits, bk = vid / p.ktiles / p.ksplits;
-    const int b = bk / p.KV, kv = bk % p.KV;
+    const int kv = vid % p.KV, kt = vid / p.KV % p.ktiles, bs = vid / p.KV / p.ktiles, split = bs % p.ksplits, b = bs / p.ksplits;
+    const int bk = b * p.KV + kv;
     const int len = image_len(p, b), key0 = kt * 32 * KW, key = key0 + 32 * kw + (lane & 31);
     const bool vis = key < len && (!p.mask || p.mask[(size_t)b * p.ldm + key]);
 
