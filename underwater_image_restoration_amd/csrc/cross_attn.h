@@ -166,6 +166,32 @@ __device__ __forceinline__ unsigned xcd_order(unsigned bid, unsigned nblocks) {
     return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + bid / 8;
 }
 
+// Which (head, image, part, tile) a block works on.  Heads next to each other: the blocks that run together read whole rows.
+// Then, an XCD taking a contiguous range of the order: with all images of one length the images far apart, so that an XCD holds
+// few images' keys in its L2; with lengths of their own next to each other, so that every XCD gets its share of the long ones.
+struct Item {
+    int kv, b, part, tile;
+};
+__device__ __forceinline__ Item block_item(unsigned vid, int KV, int B, int parts, int tiles, bool ragged) {
+    Item it;
+    it.kv = vid % KV;
+    vid /= KV;
+    if (ragged) {
+        // turned by one image per round, and by one more per round of rounds: blocks go to the CUs in turn, and a CU that met
+        // the same image every time would be done early or late
+        unsigned turn = 0;
+        if (B > 1)
+            for (unsigned t = vid / B; t; t /= B) turn += t;
+        it.b = (vid + turn) % B;
+        vid /= B;
+    }
+    it.tile = vid % tiles;
+    vid /= tiles;
+    it.part = vid % parts;
+    if (!ragged) it.b = vid / parts;
+    return it;
+}
+
 }  // namespace xattn
 
 // ---- host side: argument checks shared by both directions

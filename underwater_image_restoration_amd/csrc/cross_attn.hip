@@ -170,8 +170,8 @@ __global__ void __launch_bounds__(NW * 64, QG == 2 ? 2 : 1) xattn_tile_kernel(XA
     __shared__ __attribute__((aligned(16))) T sV[2][KT * L::STR];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const unsigned vid = xcd_order(blockIdx.x, p.nblocks);
-    // heads next to each other: the blocks that run together read whole rows
-    const int kv = vid % p.KV, qt = vid / p.KV % p.qtiles, bs = vid / p.KV / p.qtiles, split = bs % p.splits, b = bs / p.splits;
+    const Item it = block_item(vid, p.KV, p.B, p.splits, p.qtiles, p.lens != nullptr);
+    const int b = it.b, kv = it.kv, split = it.part, qt = it.tile;
     int begin, end;
     key_range(p, b, split, KT, begin, end);
 
@@ -295,7 +295,8 @@ __global__ void __launch_bounds__(256) xattn_row_kernel(XArgs p) {
     T* sK = reinterpret_cast<T*>(smem) + wave * 2 * TILE;
     T* sV = sK + TILE;
     const unsigned vid = xcd_order(blockIdx.x, p.nblocks);
-    const int kv = vid % p.KV, split = vid / p.KV % p.splits, b = vid / p.KV / p.splits;   // heads together, as above
+    const Item it = block_item(vid, p.KV, p.B, p.splits, 1, p.lens != nullptr);
+    const int b = it.b, kv = it.kv, split = it.part;
     int begin, end;
     key_range(p, b, split, 4 * KT, begin, end);
     const T* K = (const T*)p.k + (size_t)b * p.nk * p.ldk + (size_t)kv * p.hd;

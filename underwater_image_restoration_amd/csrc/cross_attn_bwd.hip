@@ -55,18 +55,17 @@ template <typename F> __device__ __forceinline__ F zero_frag() {
 
 // ---------------------------------------------------------------------------------------- dq
 template <typename T, int HD, int QG>
-__global__ void __launch_bounds__(256) xattn_dq_kernel(BArgs p) {
+__global__ void __launch_bounds__(256, QG == 2 ? 2 : 1) xattn_dq_kernel(BArgs p) {
     typedef Tile<T, HD> L;
     typedef typename L::M M;
     typedef typename M::frag frag;
     constexpr int KT = 64, NC = KT * L::CPR / 256, KS = HD / M::KSTEP, DG = HD / 32;
     __shared__ __attribute__((aligned(16))) T sK[2][KT * L::STR];
     __shared__ __attribute__((aligned(16))) T sV[2][KT * L::STR];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const unsigned vid = xcd_order(blockIdx.x, p.qblocks);
-    // heads next to each other: the blocks that run together then read whole rows (cross_attn.hip)
-    const int kv = vid % p.KV, qt = vid / p.KV % p.qtiles, bs = vid / p.KV / p.qtiles, split = bs % p.qsplits, b = bs / p.qsplits;
-    const int bk = b * p.KV + kv;
+    const Item it = block_item(vid, p.KV, p.B, p.qsplits, p.qtiles, p.lens != nullptr);
+    const int b = it.b, kv = it.kv, split = it.part, qt = it.tile, bk = b * p.KV + kv;
     int begin = 0, end = image_len(p, b);
     if (p.qsplits > 1) {
         const int tiles = (end + KT - 1) / KT, per = (tiles + p.qsplits - 1) / p.qsplits;
@@ -76,26 +75,31 @@ __global__ void __launch_bounds__(256) xattn_dq_kernel(BArgs p) {
     const T* K = (const T*)p.k + (size_t)b * p.nk * p.ldk + (size_t)kv * p.hd;
     const T* V = (const T*)p.v + (size_t)b * p.nk * p.ldv + (size_t)kv * p.hd;
     const unsigned char* mask = p.mask ? p.mask + (size_t)b * p.ldm : nullptr;
-
+    const int width = p.hd * (int)sizeof(T);
+    const size_t ldkb = p.ldk * sizeof(T), ldvb = p.ldv * sizeof(T);
+    unsigned ko[NC], vo[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        const int row = (tid + 256 * i) / L::CPR, col = (tid + 256 * i) % L::CPR * 16;
+        ko[i] = tile_offset(row, (unsigned)ldkb, col, width);
+        vo[i] = tile_offset(row, (unsigned)ldvb, col, width);
+    }
     frag rk[NC], rv[NC];
     bool vis;
     auto load = [&](int k0) {
+        const __amdgpu_buffer_rsrc_t kr = tile_buffer(K, ldkb, k0, end, width), vr = tile_buffer(V, ldvb, k0, end, width);
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
-            const int ci = tid + 256 * i, d = (ci % L::CPR) * L::VEC, key = min(k0 + ci / L::CPR, end - 1);
-            rk[i] = rv[i] = zero_frag<frag>();
-            if (d < p.hd) {
-                rk[i] = *reinterpret_cast<const frag*>(K + (size_t)key * p.ldk + d);
-                rv[i] = *reinterpret_cast<const frag*>(V + (size_t)key * p.ldv + d);
-            }
+            rk[i] = buffer_frag<frag>(kr, ko[i]);
+            rv[i] = buffer_frag<frag>(vr, vo[i]);
         }
         vis = k0 + lane < end && (!mask || mask[k0 + lane]);
     };
     auto store = [&](int buf, unsigned long long bits) {
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
-            const int ci = tid + 256 * i, row = ci / L::CPR, d = (ci % L::CPR) * L::VEC;
-            if (bits != ~0ull && !((bits >> row) & 1)) rk[i] = rv[i] = zero_frag<frag>();   // whatever hidden keys hold
+            const int row = (tid + 256 * i) / L::CPR, d = (tid + 256 * i) % L::CPR * L::VEC;
+            if (mask && !((bits >> row) & 1)) rk[i] = rv[i] = frag{};   // whatever keys hidden by the mask hold
             *reinterpret_cast<frag*>(&sK[buf][row * L::STR + d]) = rk[i];
             *reinterpret_cast<frag*>(&sV[buf][row * L::STR + d]) = rv[i];
         }
@@ -151,8 +155,6 @@ __global__ void __launch_bounds__(256) xattn_dq_kernel(BArgs p) {
         if (bits && !idle) {
 #pragma unroll
             for (int kb = 0; kb < KT / 32; ++kb) {
-                const unsigned b32 = (unsigned)(bits >> (32 * kb));
-                if (!b32) continue;
                 f32x16 s[QG], dp[QG];
 #pragma unroll
                 for (int g = 0; g < QG; ++g) {
@@ -170,23 +172,22 @@ __global__ void __launch_bounds__(256) xattn_dq_kernel(BArgs p) {
                         M::rows(dp[g], vf, fg[g][ks]);
                     }
                 }
+                const auto hider = M::hider(!(((unsigned)(bits >> (32 * kb)) >> (lane & 31)) & 1), lane);
                 typename M::Prob ds[QG];
-                const unsigned hb = b32 >> (4 * (lane >> 5));
 #pragma unroll
                 for (int g = 0; g < QG; ++g) {
+                    M::hide(s[g], hider, lane);
                     float v[16];
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        v[r] = __builtin_amdgcn_exp2f(fmaf(s[g][r], c, -l2[g])) * (dp[g][r] - D[g]);
-                        if (b32 != ~0u) v[r] = (hb >> ((r & 3) + 8 * (r >> 2))) & 1u ? v[r] : 0.f;
-                    }
+                    for (int r = 0; r < 16; ++r) v[r] = __builtin_amdgcn_exp2f(fmaf(s[g][r], c, -l2[g])) * (dp[g][r] - D[g]);
                     ds[g] = M::pack(v);
                 }
 #pragma unroll
-                for (int dg = 0; dg < DG; ++dg)
+                for (int dg = 0; dg < DG; ++dg) {
+                    const auto kt = M::template col_frags<L::STR>(&sK[buf][32 * kb * L::STR + 32 * dg], lane);
 #pragma unroll
-                    for (int g = 0; g < QG; ++g)
-                        M::template cols<L::STR>(dq[g][dg], &sK[buf][32 * kb * L::STR + 32 * dg], lane, ds[g]);
+                    for (int g = 0; g < QG; ++g) M::cols(dq[g][dg], kt, ds[g]);
+                }
             }
         }
         if (more) {
@@ -235,8 +236,8 @@ __global__ void __launch_bounds__(256) xattn_dkv_kernel(BArgs p) {
     T* sG = sQ + 2 * TILE;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, kw = wave % KW, wr = wave / KW;
     const unsigned vid = xcd_order(blockIdx.x, p.kblocks);
-    const int kv = vid % p.KV, kt = vid / p.KV % p.ktiles, bs = vid / p.KV / p.ktiles, split = bs % p.ksplits, b = bs / p.ksplits;
-    const int bk = b * p.KV + kv;
+    const Item it = block_item(vid, p.KV, p.B, p.ksplits, p.ktiles, p.lens != nullptr);
+    const int b = it.b, kv = it.kv, split = it.part, kt = it.tile, bk = b * p.KV + kv;
     const int len = image_len(p, b), key0 = kt * 32 * KW, key = key0 + 32 * kw + (lane & 31);
     const bool vis = key < len && (!p.mask || p.mask[(size_t)b * p.ldm + key]);
 
@@ -326,8 +327,8 @@ __global__ void __launch_bounds__(256) xattn_dkv_kernel(BArgs p) {
                     const f32x4 D = *reinterpret_cast<const f32x4*>(&sD[buf][32 * rb + 8 * u + 4 * (lane >> 5)]);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const float e = __builtin_amdgcn_exp2f(fmaf(s[4 * u + j], c, -l[j]));
-                        pr[4 * u + j] = vis ? e : 0.f;
+                        // (a hidden key's lane holds anything: it is a column of its own to the end)
+                        pr[4 * u + j] = __builtin_amdgcn_exp2f(fmaf(s[4 * u + j], c, -l[j]));
                         ds[4 * u + j] = pr[4 * u + j] * (dp[4 * u + j] - D[j]);
                     }
                 }
@@ -444,6 +445,7 @@ __global__ void __launch_bounds__(256) xattn_sum_rows_kernel(BArgs p) {
 
 // ---------------------------------------------------------------------------------------- launch rules
 struct Plan {
+    bool two;   // dq: two row groups a wave
     int qsplits, qtiles, kw, ksplits, ktiles;
 };
 
@@ -460,7 +462,8 @@ int parts(long long blocks, long long tiles) {
 Plan plan_bwd(int B, int nq, int nk, int H, int KV, int hd, int dtype) {
     Plan pl = {};
     const long long R = (long long)nq * (H / KV), bk = (long long)B * KV;
-    pl.qtiles = (int)((R + 127) / 128);
+    pl.two = dtype == UWIR_BF16 && hd <= 64 && R > 128 && (R + 255) / 256 * bk >= 512;
+    pl.qtiles = (int)((R + (pl.two ? 255 : 127)) / (pl.two ? 256 : 128));
     pl.qsplits = parts(bk * pl.qtiles, (nk + 63) / 64);
     // few keys: waves beyond them take rows instead (fp32 rows of 128 columns leave no LDS for the longer row tiles)
     pl.kw = hd > 64 && dtype == UWIR_F32 ? 4 : nk <= 32 ? 1 : nk <= 64 ? 2 : 4;
@@ -490,7 +493,11 @@ Layout layout(const Plan& pl, int B, int nq, int nk, int H, int KV, int hd) {
 
 template <typename T, int HD> void launch(const BArgs& p, const Plan& pl, hipStream_t st) {
     if (p.nq > 0) {
-        hipLaunchKernelGGL((xattn_dq_kernel<T, HD, 1>), dim3(p.qblocks), dim3(256), 0, st, p);
+        if (pl.two) {
+            if constexpr (sizeof(T) == 2 && HD <= 64)
+                hipLaunchKernelGGL((xattn_dq_kernel<T, HD, 2>), dim3(p.qblocks), dim3(256), 0, st, p);
+        } else
+            hipLaunchKernelGGL((xattn_dq_kernel<T, HD, 1>), dim3(p.qblocks), dim3(256), 0, st, p);
         if (p.qsplits > 1) {
             const size_t n = (size_t)p.B * p.KV * p.R * (p.hd / 8);
             hipLaunchKernelGGL((xattn_sum_rows_kernel<T>), dim3((unsigned)ceil_div_sz(n, 256)), dim3(256), 0, st, p);
