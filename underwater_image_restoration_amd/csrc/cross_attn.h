@@ -166,6 +166,18 @@ __device__ __forceinline__ unsigned xcd_order(unsigned bid, unsigned nblocks) {
     return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + bid / 8;
 }
 
+// r / G for 0 <= r < 2^30 by one high product: G in (2^(sh - 1), 2^sh], mul = floor(2^32 (2^sh - G) / G) + 1
+struct Divisor {
+    unsigned mul, sh, d;
+    __device__ __forceinline__ unsigned quot(unsigned r) const { return (__umulhi(r, mul) + r) >> sh; }
+};
+inline Divisor make_divisor(unsigned d) {
+    Divisor v = {0, 0, d};
+    while ((1u << v.sh) < d) ++v.sh;
+    v.mul = (unsigned)(((((unsigned long long)1 << v.sh) - d) << 32) / d + 1);
+    return v;
+}
+
 // Which (head, image, part, tile) a block works on.  Heads next to each other: the blocks that run together read whole rows.
 // Then, an XCD taking a contiguous range of the order: with all images of one length the images far apart, so that an XCD holds
 // few images' keys in its L2; with lengths of their own next to each other, so that every XCD gets its share of the long ones.

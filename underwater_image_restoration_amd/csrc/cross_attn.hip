@@ -23,6 +23,7 @@ struct XArgs {
     float* part_l;      // [splits][B * KV * R] log2-domain normalisers (-inf: nothing seen)
     size_t ldq, ldk, ldv, ldo, ldm;
     int B, nq, nk, H, KV, hd, G, R, splits, nblocks, qtiles;
+    Divisor by_g;
     float c;            // scale * log2(e)
 };
 
@@ -37,7 +38,7 @@ struct RowRef {
     int head;
 };
 __device__ __forceinline__ RowRef row_ref(const XArgs& p, int b, int kv, int r) {
-    const int qi = p.G == 1 ? r : r / p.G;
+    const int qi = (int)p.by_g.quot((unsigned)r);
     return {(size_t)b * p.nq + qi, kv * p.G + (r - qi * p.G)};
 }
 
@@ -515,6 +516,7 @@ extern "C" int uwir_cross_attn(const void* q, size_t ldq, const void* k, size_t 
     UWIR_CHECK(nb < (1ll << 31), "cross_attn: too many rows for one launch");
     p.nblocks = (int)nb;
     p.c = scale * LOG2E;
+    p.by_g = make_divisor(p.G);
     if (need) {
         p.part_o = (float*)workspace;
         p.part_l = (float*)((char*)workspace + al256((size_t)pl.splits * B * heads * nq * hd * 4));

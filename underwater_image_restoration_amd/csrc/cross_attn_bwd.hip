@@ -25,6 +25,7 @@ struct BArgs {
     int B, nq, nk, H, KV, hd, G, R;
     int qsplits, qtiles, qblocks;  // rows kernel
     int ksplits, ktiles, kblocks;  // keys kernel
+    Divisor by_g;
     float c, scale;
 };
 
@@ -38,19 +39,12 @@ struct RowRef {
     int head;
 };
 __device__ __forceinline__ RowRef row_ref(const BArgs& p, int b, int kv, int r) {
-    const int qi = p.G == 1 ? r : r / p.G;
+    const int qi = (int)p.by_g.quot((unsigned)r);
     return {(size_t)b * p.nq + qi, kv * p.G + (r - qi * p.G)};
 }
 
 __device__ __forceinline__ int image_len(const BArgs& p, int b) {
     return p.lens ? max(0, min(p.nk, p.lens[b])) : p.nk;
-}
-
-template <typename F> __device__ __forceinline__ F zero_frag() {
-    F f;
-#pragma unroll
-    for (int j = 0; j < (int)(sizeof(F) / sizeof(f[0])); ++j) f[j] = 0;
-    return f;
 }
 
 // ---------------------------------------------------------------------------------------- dq
@@ -121,7 +115,7 @@ __global__ void __launch_bounds__(256, QG == 2 ? 2 : 1) xattn_dq_kernel(BArgs p)
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             const int d = ks * M::KSTEP + (lane >> 5) * M::VEC;
-            fq[g][ks] = fg[g][ks] = zero_frag<frag>();
+            fq[g][ks] = fg[g][ks] = frag{};
             if (ok && d < p.hd) {
                 fq[g][ks] = *reinterpret_cast<const frag*>(Q + d);
                 fg[g][ks] = *reinterpret_cast<const frag*>(GO + d);
@@ -238,47 +232,29 @@ __global__ void __launch_bounds__(256) xattn_dkv_kernel(BArgs p) {
     const unsigned vid = xcd_order(blockIdx.x, p.kblocks);
     const Item it = block_item(vid, p.KV, p.B, p.ksplits, p.ktiles, p.lens != nullptr);
     const int b = it.b, kv = it.kv, split = it.part, kt = it.tile, bk = b * p.KV + kv;
-    const int len = image_len(p, b), key0 = kt * 32 * KW, key = key0 + 32 * kw + (lane & 31);
-    const bool vis = key < len && (!p.mask || p.mask[(size_t)b * p.ldm + key]);
-
-    frag fk[KS], fv[KS];
-    f32x16 dk[DG], dv[DG];
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-        const int d = ks * M::KSTEP + (lane >> 5) * M::VEC;
-        fk[ks] = fv[ks] = zero_frag<frag>();
-        if (vis && d < p.hd) {
-            fk[ks] = *reinterpret_cast<const frag*>((const T*)p.k + ((size_t)b * p.nk + key) * p.ldk + (size_t)kv * p.hd + d);
-            fv[ks] = *reinterpret_cast<const frag*>((const T*)p.v + ((size_t)b * p.nk + key) * p.ldv + (size_t)kv * p.hd + d);
-        }
-    }
-#pragma unroll
-    for (int dg = 0; dg < DG; ++dg) {
-        zero16(dk[dg]);
-        zero16(dv[dg]);
-    }
     int begin = 0, end = p.R;
     if (p.ksplits > 1) {
         const int tiles = (p.R + RT - 1) / RT, per = (tiles + p.ksplits - 1) / p.ksplits;
         begin = min(p.R, split * per * RT);
         end = min(p.R, (split + 1) * per * RT);
     }
-    // a block whose keys are all hidden has nothing to add up (block-uniform, ahead of every barrier but this one)
-    if (!__syncthreads_or(vis)) end = begin;
-    const bool idle = !__any(vis);
-
     frag rq[NC], rg[NC];
     float2 rl;
+    const int width = p.hd * (int)sizeof(T);
+    const size_t ldqb = p.ldq * sizeof(T), ldgb = p.ldg * sizeof(T);
+    const T* Q = (const T*)p.q + (size_t)b * p.nq * p.ldq + (size_t)kv * p.G * p.hd;
+    const T* GO = (const T*)p.go + (size_t)b * p.nq * p.ldg + (size_t)kv * p.G * p.hd;
+    // a tile's packed rows lie in the rows from the first one's query on, G heads side by side: a buffer at that query
     auto load = [&](int r0) {
+        const int q0 = (int)p.by_g.quot((unsigned)r0);
+        const __amdgpu_buffer_rsrc_t qb = tile_buffer(Q, ldqb, q0, p.nq, width * p.G), gb = tile_buffer(GO, ldgb, q0, p.nq, width * p.G);
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
-            const int ci = tid + 256 * i, d = (ci % L::CPR) * L::VEC, r = r0 + ci / L::CPR;
-            rq[i] = rg[i] = zero_frag<frag>();
-            if (r < end && d < p.hd) {
-                const RowRef f = row_ref(p, b, kv, r);
-                rq[i] = *reinterpret_cast<const frag*>((const T*)p.q + f.row * p.ldq + (size_t)f.head * p.hd + d);
-                rg[i] = *reinterpret_cast<const frag*>((const T*)p.go + f.row * p.ldg + (size_t)f.head * p.hd + d);
-            }
+            const int ci = tid + 256 * i, col = ci % L::CPR * 16, r = r0 + ci / L::CPR;
+            const unsigned qi = p.by_g.quot((unsigned)r), in_row = (r - qi * p.G) * width + col;
+            const bool ok = r < end && col < width;
+            rq[i] = buffer_frag<frag>(qb, ok ? (qi - q0) * (unsigned)ldqb + in_row : 0x80000000u);
+            rg[i] = buffer_frag<frag>(gb, ok ? (qi - q0) * (unsigned)ldgb + in_row : 0x80000000u);
         }
         rl = make_float2(0.f, 0.f);
         if (tid < RT && r0 + tid < end) rl = p.ld[(size_t)bk * p.R + r0 + tid];
@@ -295,11 +271,35 @@ __global__ void __launch_bounds__(256) xattn_dkv_kernel(BArgs p) {
             sD[buf][tid] = rl.y;
         }
     };
-    const float c = p.c;
-    if (begin < end) {
-        load(begin);
-        store(0);
+    // rows, keys and mask are asked for together: one latency, not three in a row
+    if (begin < end) load(begin);
+    const int key = kt * 32 * KW + 32 * kw + (lane & 31), krow = min(key, p.nk - 1);
+    frag fk[KS], fv[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        const int d = ks * M::KSTEP + (lane >> 5) * M::VEC;
+        fk[ks] = fv[ks] = frag{};
+        if (d < p.hd) {
+            fk[ks] = *reinterpret_cast<const frag*>((const T*)p.k + ((size_t)b * p.nk + krow) * p.ldk + (size_t)kv * p.hd + d);
+            fv[ks] = *reinterpret_cast<const frag*>((const T*)p.v + ((size_t)b * p.nk + krow) * p.ldv + (size_t)kv * p.hd + d);
+        }
     }
+    const bool shown = !p.mask || p.mask[(size_t)b * p.ldm + krow], vis = key < image_len(p, b) && shown;
+    f32x16 dk[DG], dv[DG];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+        if (!vis) fk[ks] = fv[ks] = frag{};
+#pragma unroll
+    for (int dg = 0; dg < DG; ++dg) {
+        zero16(dk[dg]);
+        zero16(dv[dg]);
+    }
+    // a block whose keys are all hidden has nothing to add up
+    if (!__syncthreads_or(vis)) end = begin;
+    const bool idle = !__any(vis);
+
+    const float c = p.c;
+    if (begin < end) store(0);
     __syncthreads();
     int buf = 0;
     for (int r0 = begin; r0 < end; r0 += RT, buf ^= 1) {
@@ -459,12 +459,15 @@ int parts(long long blocks, long long tiles) {
     return s < 1 ? 1 : (int)s;
 }
 
-Plan plan_bwd(int B, int nq, int nk, int H, int KV, int hd, int dtype) {
+Plan plan_bwd(int B, int nq, int nk, int H, int KV, int hd, int dtype, bool ragged) {
     Plan pl = {};
-    const long long R = (long long)nq * (H / KV), bk = (long long)B * KV;
-    pl.two = dtype == UWIR_BF16 && hd <= 64 && R > 128 && (R + 255) / 256 * bk >= 512;
+    const long long R = (long long)nq * (H / KV), bk = (long long)B * KV, wide = (R + 255) / 256 * bk;
+    pl.qsplits = parts(bk * ((R + 127) / 128), (nk + 63) / 64);
+    // 256 rows a block (bf16, up to 64 columns) where two such blocks a CU remain; with lengths per image, where the longest image's
+    // blocks set the time, only from eight on.  4 x 64 x 64 queries over 2048 states, 8 heads of 64: 273 against 310 us; ragged and
+    // with shared heads 248 against 241.
+    pl.two = dtype == UWIR_BF16 && hd <= 64 && R > 128 && pl.qsplits == 1 && wide >= (ragged ? 2048 : 512);
     pl.qtiles = (int)((R + (pl.two ? 255 : 127)) / (pl.two ? 256 : 128));
-    pl.qsplits = parts(bk * pl.qtiles, (nk + 63) / 64);
     // few keys: waves beyond them take rows instead (fp32 rows of 128 columns leave no LDS for the longer row tiles)
     pl.kw = hd > 64 && dtype == UWIR_F32 ? 4 : nk <= 32 ? 1 : nk <= 64 ? 2 : 4;
     pl.ktiles = (nk + 32 * pl.kw - 1) / (32 * pl.kw);
@@ -520,7 +523,8 @@ template <typename T, int HD> void launch(const BArgs& p, const Plan& pl, hipStr
 
 extern "C" size_t uwir_cross_attn_backward_workspace_bytes(int B, int nq, int nk, int heads, int kv_heads, int hd, int dtype) {
     if (B <= 0 || nq < 0 || nk < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || hd <= 0) return 0;
-    return layout(plan_bwd(B, nq, nk, heads, kv_heads, hd, dtype), B, nq, nk, heads, kv_heads, hd).total;
+    return layout(plan_bwd(B, nq, nk, heads, kv_heads, hd, dtype, false), B,   // the parts do not depend on the lengths
+                   nq, nk, heads, kv_heads, hd).total;
 }
 
 extern "C" int uwir_cross_attn_backward(const void* q, size_t ldq, const void* k, size_t ldk, const void* v, size_t ldv,
@@ -541,7 +545,7 @@ extern "C" int uwir_cross_attn_backward(const void* q, size_t ldq, const void* k
     const size_t need = uwir_cross_attn_backward_workspace_bytes(B, nq, nk, heads, kv_heads, hd, dtype);
     UWIR_CHECK(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
                "cross_attn_backward: workspace too small or not 16-byte aligned");
-    const Plan pl = plan_bwd(B, nq, nk, heads, kv_heads, hd, dtype);
+    const Plan pl = plan_bwd(B, nq, nk, heads, kv_heads, hd, dtype, key_lens != nullptr);
     const Layout lo = layout(pl, B, nq, nk, heads, kv_heads, hd);
     BArgs p = {};
     p.q = q; p.k = k; p.v = v; p.o = out; p.go = dout; p.lse = lse; p.dq = dq; p.dk = dk; p.dv = dv;
@@ -553,7 +557,7 @@ extern "C" int uwir_cross_attn_backward(const void* q, size_t ldq, const void* k
     const long long qb = (long long)B * kv_heads * pl.qtiles * pl.qsplits, kb = (long long)B * kv_heads * pl.ktiles * pl.ksplits;
     UWIR_CHECK(qb < (1ll << 31) && kb < (1ll << 31), "cross_attn_backward: too many rows for one launch");
     p.qblocks = (int)qb; p.kblocks = (int)kb;
-    p.c = scale * LOG2E; p.scale = scale;
+    p.c = scale * LOG2E; p.scale = scale; p.by_g = make_divisor(p.G);
     char* ws = (char*)workspace;
     p.ld = (float2*)(ws + lo.ld);
     p.part_q = (float*)(ws + lo.q); p.part_k = (float*)(ws + lo.k); p.part_v = (float*)(ws + lo.v);
