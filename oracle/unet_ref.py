@@ -128,7 +128,9 @@ def unet_forward(sd: SD, xt: torch.Tensor, cond: torch.Tensor, time, text_contex
                       sd["text_mlp.2.weight"], sd["text_mlp.2.bias"])
         pe = torch.softmax(pe, dim=1) * sd["prompt"]
         t = t + F.linear(pe, sd["prompt_mlp.weight"], sd["prompt_mlp.bias"])
-    ctx = image_context.unsqueeze(1) if image_context is not None else None         # :139-140
+    ctx = image_context                                                               # :139-140; (B, L, D): L states
+    if ctx is not None and ctx.dim() == 2:
+        ctx = ctx.unsqueeze(1)
     if taps is not None:
         taps["t"], taps["init"] = t, x
     hs: List[torch.Tensor] = []

@@ -17,6 +17,9 @@ Everything runs NHWC through the C ABI (include/uwir.h); this file owns buffers,
   * LinearAttention = 3 HBM passes (uwir_linear_attention); SpatialTransformer = GroupNorm folded into the
     proj_in GEMM, flash attention, cross-attention on the single context token collapsed to a per-sample bias
     (softmax over one key is 1: attention.py:176-190 with context (B,1,512)), GEGLU.
+  * ``image_context`` may also be the encoder's states, (B, L, context_dim) with L of its own (attention.py:176-190 takes any
+    length), each image's count in ``context_lens``: the norm is then one pass (uwir_group_norm_act) and the second attention
+    a cross attention over the states (uwir_cross_attn).
 """
 from __future__ import annotations
 
@@ -160,6 +163,10 @@ class ConditionalUNet(nn.Module):
                      w_in=conv(sd[f + "proj_in.weight"]), b_in=vec(sd[f + "proj_in.bias"]),
                      w_qkv=torch.cat([sd[t + "attn1.to_q.weight"], sd[t + "attn1.to_k.weight"],
                                       sd[t + "attn1.to_v.weight"]], dim=0).to(wdt).contiguous(), qcs=cs,
+                     w_q2=sd[t + "attn2.to_q.weight"].to(wdt).contiguous(),
+                     w_kv2=torch.cat([sd[t + "attn2.to_k.weight"], sd[t + "attn2.to_v.weight"]], dim=0).to(wdt).contiguous(),
+                     w_o2=sd[t + "attn2.to_out.0.weight"].to(wdt).contiguous(), b_o2=vec(sd[t + "attn2.to_out.0.bias"]),
+                     n2=(vec(sd[t + "norm2.weight"]), vec(sd[t + "norm2.bias"])),
                      w_o1=sd[t + "attn1.to_out.0.weight"].to(wdt).contiguous(), b_o1=vec(sd[t + "attn1.to_out.0.bias"]),
                      n1=(vec(sd[t + "norm1.weight"]), vec(sd[t + "norm1.bias"])),
                      n3=(vec(sd[t + "norm3.weight"]), vec(sd[t + "norm3.bias"])),
@@ -255,8 +262,9 @@ class ConditionalUNet(nn.Module):
             ops.conv_gemm(x, r["wres"], res, B=B, H=H, W=W, C_=din, N=dout)
         ops.conv_gemm(h, r["w2"], out, B=B, H=H, W=W, C_=dout, N=dout, KH=3, KW=3, pad=1, act=ops.ACT_SILU, res=res)
 
-    def _attn(self, a: dict, x: torch.Tensor, out: torch.Tensor, B: int, H: int, W: int, u_all, tag: str):
-        """Residual(PreNorm(dim, LinearAttention | SpatialTransformer)): x [M, dim] view -> out [M, dim] view."""
+    def _attn(self, a: dict, x: torch.Tensor, out: torch.Tensor, B: int, H: int, W: int, u_all, tag: str, states=None):
+        """Residual(PreNorm(dim, LinearAttention | SpatialTransformer)): x [M, dim] view -> out [M, dim] view.  ``states``: None,
+        or the encoder's states as (rows [B * L, context_dim], L, lens int32 [B] or None)."""
         M, n, dev, adt, f32 = B * H * W, H * W, x.device, self._pack["adt"], torch.float32
         dim = a["g_pre"].numel()
         if a["kind"] == "linear" and adt == torch.bfloat16 and dim in (64, 128, 256) and self.fused_linattn:
@@ -280,16 +288,22 @@ class ConditionalUNet(nn.Module):
                 ops.ln_rows(y, a["g_out"], None, y, 1e-5)
                 ops.add_rows(y, x, out)
             return
-        if u_all is None:
+        if u_all is None and states is None:
             raise ValueError("image_context is required: the model was built with use_image_context=True")
         heads = a["heads"]
         xn = self._buf(tag + "xn", M, dim, f32, dev)
         ops.ln_rows(x, a["g_pre"], None, xn, 1e-5)
-        ga, gs = self._buf(tag + "ga", B, dim, f32, dev), self._buf(tag + "gs", B, dim, f32, dev)
-        ws = self._buf("gn_ws", 1, max(ops.ln2d_workspace_bytes(B, n, dim) // 8, 1), torch.float64, dev)
-        ops.groupnorm_affine(xn, B, n, dim, 32, 1e-6, a["gn_w"], a["gn_b"], ga, gs, ws)
         t0 = self._buf(tag + "t0", M, dim, f32, dev)
-        ops.conv_gemm(xn, a["w_in"], t0, B=B, H=H, W=W, C_=dim, N=dim, a_scale=ga, a_shift=gs, bias=a["b_in"])
+        if states is None:
+            ga, gs = self._buf(tag + "ga", B, dim, f32, dev), self._buf(tag + "gs", B, dim, f32, dev)
+            ws = self._buf("gn_ws", 1, max(ops.ln2d_workspace_bytes(B, n, dim) // 8, 1), torch.float64, dev)
+            ops.groupnorm_affine(xn, B, n, dim, 32, 1e-6, a["gn_w"], a["gn_b"], ga, gs, ws)
+            ops.conv_gemm(xn, a["w_in"], t0, B=B, H=H, W=W, C_=dim, N=dim, a_scale=ga, a_shift=gs, bias=a["b_in"])
+        else:
+            xg = self._buf(tag + "xg", M, dim, adt, dev)
+            ws = self._buf(tag + "gna_ws", 1, ops.group_norm_act_workspace_bytes(B, n, dim, 32), torch.uint8, dev)
+            ops.group_norm_act(xn, B, n, dim, 32, 1e-6, a["gn_w"], a["gn_b"], xg, ws)
+            ops.conv_gemm(xg, a["w_in"], t0, B=B, H=H, W=W, C_=dim, N=dim, bias=a["b_in"])
         h = self._buf(tag + "h", M, dim, adt, dev)
         ops.ln_rows(t0, a["n1"][0], a["n1"][1], h, 1e-5)
         qkv = self._buf(tag + "qkv", M, 3 * dim, adt, dev)
@@ -297,8 +311,21 @@ class ConditionalUNet(nn.Module):
         att = self._buf(tag + "att", M, dim, adt, dev)
         ops.flash_attn(qkv[:, :dim], qkv[:, dim:2 * dim], qkv[:, 2 * dim:], None, B, n, heads, 32, 0.0, att, None)
         t1 = self._buf(tag + "t1", M, dim, f32, dev)
-        o = a["ov_off"]
-        ops.conv_gemm(att, a["w_o1"], t1, B=B, H=H, W=W, C_=dim, N=dim, bias=a["b_o1"], batch_bias=u_all[:, o:o + dim], res=t0)
+        if states is None:
+            o = a["ov_off"]
+            ops.conv_gemm(att, a["w_o1"], t1, B=B, H=H, W=W, C_=dim, N=dim, bias=a["b_o1"], batch_bias=u_all[:, o:o + dim], res=t0)
+        else:
+            rows, L, lens = states
+            s1 = self._buf(tag + "s1", M, dim, f32, dev)
+            ops.conv_gemm(att, a["w_o1"], s1, B=B, H=H, W=W, C_=dim, N=dim, bias=a["b_o1"], res=t0)
+            ops.ln_rows(s1, a["n2"][0], a["n2"][1], h, 1e-5)
+            q2, kv2 = self._buf(tag + "q2", M, dim, adt, dev), self._buf(tag + "kv2", B * L, 2 * dim, adt, dev)
+            ops.gemm(h, a["w_q2"], q2)
+            ops.gemm(rows, a["w_kv2"], kv2)
+            nb = ops.cross_attn_workspace_bytes(B, n, L, heads, heads, 32, adt)
+            ws = self._buf(tag + "xa_ws", 1, nb, torch.uint8, dev) if nb else None
+            ops.cross_attn(q2, kv2[:, :dim], kv2[:, dim:], B, n, L, heads, heads, 32, 32 ** -0.5, att, ws, key_lens=lens)
+            ops.conv_gemm(att, a["w_o2"], t1, B=B, H=H, W=W, C_=dim, N=dim, bias=a["b_o2"], res=s1)
         ops.ln_rows(t1, a["n3"][0], a["n3"][1], h, 1e-5)
         gg = self._buf(tag + "gg", M, 4 * dim, adt, dev)     # GEGLU in the projection's epilogue (rows paired by _build_pack)
         ops.conv_gemm(h, a["w_ff0"], gg, B=B, H=H, W=W, C_=dim, N=8 * dim, bias=a["b_ff0"], store_mode=2)
@@ -331,7 +358,7 @@ class ConditionalUNet(nn.Module):
         ss_all = self._buf(tag + "ss_all", R, pk["ss_w"].shape[0], f32, dev)
         ops.linear(st, pk["ss_w"], pk["ss_b"], ss_all)
         u_all = None
-        if "ov_w" in pk and self._has_st and image_context is not None:
+        if "ov_w" in pk and self._has_st and image_context is not None and image_context.dim() == 2:
             u_all = self._buf(tag + "u_all", B, pk["ov_w"].shape[0], f32, dev)
             ops.linear(image_context.contiguous().float(), pk["ov_w"], pk["ov_b"], u_all)
         return ss_all, u_all, st
@@ -347,6 +374,22 @@ class ConditionalUNet(nn.Module):
         emb = self._time_embedding(time, B, dev)
         ss_all, u_all, _ = self._conditioning_rows(emb, B, B, text_context, image_context, dev, "")
         return ss_all, u_all
+
+    def _states(self, image_context, context_lens, B: int):
+        """An (B, L, context_dim) context as (rows in the GEMMs' operand type, L, lens); None for the reference's (B, context_dim)."""
+        if image_context is None or image_context.dim() == 2:
+            if context_lens is not None:
+                raise ValueError("context_lens goes with an image_context of states, (B, L, context_dim)")
+            return None
+        if image_context.dim() != 3 or image_context.shape[0] != B or image_context.shape[2] != self.context_dim or not image_context.shape[1]:
+            raise ValueError(f"image_context must be (B, {self.context_dim}) or (B, L, {self.context_dim})")
+        if self.context_dim % 8:
+            raise ValueError("an image_context of states needs context_dim % 8 == 0")
+        if context_lens is not None and (context_lens.dtype != torch.int32 or tuple(context_lens.shape) != (B,)
+                                         or context_lens.device != image_context.device):
+            raise ValueError("context_lens must be int32 [B] on the context's device")
+        rows = image_context.reshape(-1, self.context_dim).to(self._pack["adt"]).contiguous()
+        return rows, image_context.shape[1], None if context_lens is None else context_lens.contiguous()
 
     @staticmethod
     def _ctx_versions(*ts):
@@ -383,7 +426,10 @@ class ConditionalUNet(nn.Module):
     @torch.no_grad()
     @ops.on_operand_device
     def forward(self, xt: torch.Tensor, cond: torch.Tensor, time, text_context: Optional[torch.Tensor] = None,
-                image_context: Optional[torch.Tensor] = None, taps: Optional[dict] = None) -> torch.Tensor:
+                image_context: Optional[torch.Tensor] = None, taps: Optional[dict] = None,
+                context_lens: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """``image_context``: (B, context_dim), or the encoder's states (B, L, context_dim), of which image b shows the first
+        ``context_lens[b]`` (int32 [B] on the device, all L without it)."""
         if not xt.is_cuda:
             raise RuntimeError("ConditionalUNet (MI355X build) runs on a ROCm device only; there is no CPU fallback")
         if xt.dim() != 4 or xt.shape != cond.shape or xt.shape[1] != self.in_nc:
@@ -399,6 +445,8 @@ class ConditionalUNet(nn.Module):
             raise ValueError("image too small for reflect padding")
         nf, td, lv, D = self.nf, 4 * self.nf, self._levels(), self.depth
         xt, cond = xt.contiguous().float(), cond.contiguous().float()
+
+        states = self._states(image_context, context_lens, B)
 
         # ---- time / prompt embedding -> SiLU(t) -> all ResBlock (scale+1 | shift) vectors in one linear (or this
         # step's rows of a schedule computed once for the whole sampling loop: conditioning_schedule)
@@ -433,7 +481,7 @@ class ConditionalUNet(nn.Module):
             self._resblock(d["b1"], x, h1, B, Hs[i], Ws[i], ss_all, f"d{i}a")
             tmp = self._buf(f"d{i}t", Ms[i], din, sdt, dev)
             self._resblock(d["b2"], h1, tmp, B, Hs[i], Ws[i], ss_all, f"d{i}b")
-            self._attn(d["attn"], tmp, h2, B, Hs[i], Ws[i], u_all, f"d{i}c")
+            self._attn(d["attn"], tmp, h2, B, Hs[i], Ws[i], u_all, f"d{i}c", states)
             if taps is not None:
                 taps[f"down{i}"] = self._nchw(h2, B, Hs[i], Ws[i])
             if i != D - 1:
@@ -447,7 +495,7 @@ class ConditionalUNet(nn.Module):
         Hm, Wm, Mm, dm = Hs[-1], Ws[-1], Ms[-1], lv[-1][1]
         m1, m2 = self._buf("m1", Mm, dm, sdt, dev), self._buf("m2", Mm, dm, sdt, dev)
         self._resblock(pk["mid1"], x, m1, B, Hm, Wm, ss_all, "m1")
-        self._attn(pk["mid_attn"], m1, m2, B, Hm, Wm, u_all, "ma")
+        self._attn(pk["mid_attn"], m1, m2, B, Hm, Wm, u_all, "ma", states)
         self._resblock(pk["mid2"], m2, catA[D - 1][:, :dm], B, Hm, Wm, ss_all, "m2")
         if taps is not None:
             taps["mid"] = self._nchw(catA[D - 1][:, :dm], B, Hm, Wm)
@@ -458,7 +506,7 @@ class ConditionalUNet(nn.Module):
             self._resblock(u["b1"], catA[i], catB[i][:, :dout], B, Hs[i], Ws[i], ss_all, f"u{j}a")
             t2, t3 = self._buf(f"u{j}t2", Ms[i], dout, sdt, dev), self._buf(f"u{j}t3", Ms[i], dout, sdt, dev)
             self._resblock(u["b2"], catB[i], t2, B, Hs[i], Ws[i], ss_all, f"u{j}b")
-            self._attn(u["attn"], t2, t3, B, Hs[i], Ws[i], u_all, f"u{j}c")
+            self._attn(u["attn"], t2, t3, B, Hs[i], Ws[i], u_all, f"u{j}c", states)
             if taps is not None:
                 taps[f"up{j}"] = self._nchw(t3, B, Hs[i], Ws[i])
             if i != 0:
