@@ -139,7 +139,8 @@ def check(ops, t, dims, grads=True):
 # and not; splits of the key axis (few rows) and of the row axis (few keys)
 DIMS = [(1, 1, 1, 1, 1, 8), (2, 1, 77, 8, 8, 32), (3, 5, 33, 6, 2, 16), (2, 33, 1, 4, 4, 24), (3, 130, 50, 4, 4, 32), (2, 100, 64, 2, 1, 40),
         (3, 64, 65, 8, 2, 64), (2, 257, 200, 3, 1, 80), (1, 31, 129, 2, 2, 96), (3, 70, 300, 4, 2, 128), (4, 1, 5000, 8, 2, 64),
-        (1, 1, 3001, 1, 1, 128), (1, 300, 2100, 4, 2, 64), (1, 2600, 20, 2, 2, 32), (1, 3000, 61, 1, 1, 64), (1, 2000, 30, 1, 1, 128)]
+        (1, 1, 3001, 1, 1, 128), (1, 300, 2100, 4, 2, 64), (1, 2600, 20, 2, 2, 32), (1, 3000, 61, 1, 1, 64), (1, 2000, 30, 1, 1, 128),
+        (2, 300, 128, 4, 2, 32), (2, 700, 97, 2, 1, 24), (2, 500, 30, 2, 2, 64), (16, 700, 90, 4, 4, 32)]
 
 
 @pytest.mark.parametrize("keys", ["none", "lens", "mask", "both"])

@@ -1,6 +1,6 @@
 // Cross attention, backward.  With s = scale q k^T over the visible keys and p = exp(s - lse):
 //   D = sum_d dout out,  dv = p^T dout,  dp = dout v^T,  ds = p (dp - D),  dq = scale ds k,  dk = scale ds^T q
-// Two kernels, each of which keeps its result in registers and forms p again (7 products instead of the 5 that one kernel
+// More than a few keys take two kernels, each of which keeps its result in registers and forms p again (7 products instead of the 5 that one kernel
 // with both results would need; in exchange nothing is accumulated through memory in an order that changes):
 //   rows kernel  a wave owns 32 packed rows (cross_attn.hip), walks the keys: S^T = K q^T, dP^T = V dout^T,
 //                dq^T += K^T dS; also forms D and hands (lse, D) to the next kernel in packed-row order
@@ -397,6 +397,224 @@ __global__ void __launch_bounds__(256) xattn_dkv_kernel(BArgs p) {
         }
 }
 
+// ---------------------------------------------------------------------------------------- few keys: all three at once
+// Up to 32 NKB keys (captions, ViT states): K and V of a key head stay in LDS, its dk and dv in registers, and every row of q,
+// out and dout is read once.  Per unit (32 rows x 32 keys): S^T = K q^T and dP^T = V dout^T from LDS and registers, dq^T += K^T dS
+// from registers; P and dS go through a patch of LDS of the wave's own and come back transposed for dv^T += dout^T P and
+// dk^T += q^T dS.  5 products instead of 7.  The four waves' dk, dv (and the parts over blocks) are summed in order at the end.
+// Against the two kernels below it: 8 x 64 x 64 queries over 77 states, 8 heads of 32, 53 -> 33 us; over 50, 8 heads of 64, 66 -> 47 us.
+template <int HD, int NKB>
+__global__ void __launch_bounds__(256, 2) xattn_short_bwd_kernel(BArgs p) {
+    typedef bf16_t T;
+    typedef Tile<T, HD> L;
+    typedef Mma<T> M;
+    typedef M::frag frag;
+    constexpr int KS = HD / 16, DG = HD / 32, STR = L::STR, PSTR = 32 + M::PAD, JSTR = HD + 4;
+    constexpr int KVT = NKB * 32 * STR, WT = 2 * 32 * STR + 2 * 32 * PSTR;   // elements: K (or V), a wave's patch
+    constexpr int LOOP = (2 * KVT + 4 * WT) * 2, JOIN = 2 * 4 * 32 * JSTR * 4;
+    constexpr bool AHEAD = NKB * DG < 4;   // registers left to fetch the next rows while these are worked on
+    __shared__ __attribute__((aligned(16))) char smem[LOOP > JOIN ? LOOP : JOIN];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    T* sK = reinterpret_cast<T*>(smem);
+    T* sV = sK + KVT;
+    T* sQ = sV + KVT + wave * WT;
+    T* sG = sQ + 32 * STR;
+    T* sP = sG + 32 * STR;
+    T* sS = sP + 32 * PSTR;
+    const unsigned vid = xcd_order(blockIdx.x, p.kblocks);
+    const Item it = block_item(vid, p.KV, p.B, p.ksplits, 1, p.lens != nullptr);
+    const int b = it.b, kv = it.kv, split = it.part, row = lane & 31, half = lane >> 5;
+    const int steps = (p.R + 127) / 128, per = (steps + p.ksplits - 1) / p.ksplits;
+    const int begin = min(p.R, split * per * 128), end = min(p.R, (split + 1) * per * 128);
+
+    frag fq[KS], fg[KS], fo[KS];
+    float l2 = 0.f;
+    auto fetch = [&](int r) {   // row r of q, dout, out and its lse; zeros behind the last row
+        const bool ok = r < end;
+        const RowRef f = row_ref(p, b, kv, ok ? r : 0);
+        const T* Q = (const T*)p.q + f.row * p.ldq + (size_t)f.head * p.hd;
+        const T* GO = (const T*)p.go + f.row * p.ldg + (size_t)f.head * p.hd;
+        const T* O = (const T*)p.o + f.row * p.ldo + (size_t)f.head * p.hd;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const int d = ks * 16 + half * 8;
+            fq[ks] = fg[ks] = fo[ks] = frag{};
+            if (ok && d < p.hd) {
+                fq[ks] = *reinterpret_cast<const frag*>(Q + d);
+                fg[ks] = *reinterpret_cast<const frag*>(GO + d);
+                fo[ks] = *reinterpret_cast<const frag*>(O + d);
+            }
+        }
+        l2 = ok ? p.lse[((size_t)b * p.H + f.head) * p.nq + (f.row - (size_t)b * p.nq)] : 0.f;
+    };
+    int r0 = begin + wave * 32;
+    if (AHEAD && r0 < end) fetch(r0 + row);
+    // ---- keys of the whole image
+    const int len = image_len(p, b);
+    const unsigned char* mask = p.mask ? p.mask + (size_t)b * p.ldm : nullptr;
+    {
+        const T* K = (const T*)p.k + (size_t)b * p.nk * p.ldk + (size_t)kv * p.hd;
+        const T* V = (const T*)p.v + (size_t)b * p.nk * p.ldv + (size_t)kv * p.hd;
+        for (int i = tid; i < NKB * 32 * L::CPR; i += 256) {
+            const int key = i / L::CPR, d = i % L::CPR * 8;
+            frag a = frag{}, c = frag{};
+            if (key < len && d < p.hd && (!mask || mask[key])) {
+                a = *reinterpret_cast<const frag*>(K + (size_t)key * p.ldk + d);
+                c = *reinterpret_cast<const frag*>(V + (size_t)key * p.ldv + d);
+            }
+            *reinterpret_cast<frag*>(sK + key * STR + d) = a;
+            *reinterpret_cast<frag*>(sV + key * STR + d) = c;
+        }
+    }
+    unsigned hidden = 0;   // bit kb: this lane's key of block kb
+#pragma unroll
+    for (int kb = 0; kb < NKB; ++kb) {
+        const int key = 32 * kb + row;
+        if (!(key < len && (!mask || mask[key]))) hidden |= 1u << kb;
+    }
+    __syncthreads();
+
+    f32x16 dk[NKB][DG], dv[NKB][DG];
+#pragma unroll
+    for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+        for (int dg = 0; dg < DG; ++dg) {
+            zero16(dk[kb][dg]);
+            zero16(dv[kb][dg]);
+        }
+    const float c = p.c;
+    for (; r0 < end; r0 += 128) {
+        // ---- this group's rows: D, q and dout into the wave's patch
+        if (!AHEAD) fetch(r0 + row);
+        float dd = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) dd = fmaf((float)fg[ks][j], (float)fo[ks][j], dd);
+        const float2 hs = both_halves(dd);
+        const float D = hs.x + hs.y, lr = l2 == -INFINITY ? 0.f : l2 * LOG2E;
+        frag q[KS], g[KS];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            q[ks] = fq[ks];
+            g[ks] = fg[ks];
+            *reinterpret_cast<frag*>(sQ + row * STR + ks * 16 + half * 8) = q[ks];
+            *reinterpret_cast<frag*>(sG + row * STR + ks * 16 + half * 8) = g[ks];
+        }
+        if (AHEAD && r0 + 128 < end) fetch(r0 + 128 + row);
+        f32x16 dq[DG];
+#pragma unroll
+        for (int dg = 0; dg < DG; ++dg) zero16(dq[dg]);
+#pragma unroll
+        for (int kb = 0; kb < NKB; ++kb) {
+            f32x16 s, dp;
+            zero16(s);
+            zero16(dp);
+            const int off = (32 * kb + row) * STR + half * 8;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                M::rows(s, *reinterpret_cast<const frag*>(sK + off + ks * 16), q[ks]);
+                M::rows(dp, *reinterpret_cast<const frag*>(sV + off + ks * 16), g[ks]);
+            }
+            M::hide(s, M::hider((hidden >> kb) & 1, lane), lane);
+            float pr[16], ds[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                pr[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lr));
+                ds[r] = pr[r] * (dp[r] - D);
+            }
+            const M::Prob pp = M::pack(pr), pd = M::pack(ds);
+#pragma unroll
+            for (int dg = 0; dg < DG; ++dg) M::cols<STR>(dq[dg], sK + 32 * kb * STR + 32 * dg, lane, pd);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {   // quad u of the registers: keys 8 u + 4 half + 0..3 of this lane's row
+                bf16x4 a, e;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    a[j] = pp.p[u >> 1][4 * (u & 1) + j];
+                    e[j] = pd.p[u >> 1][4 * (u & 1) + j];
+                }
+                *reinterpret_cast<bf16x4*>(sP + row * PSTR + 8 * u + 4 * half) = a;
+                *reinterpret_cast<bf16x4*>(sS + row * PSTR + 8 * u + 4 * half) = e;
+            }
+            // the wave's own LDS operations stay in order; only the compiler has to be held
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            const M::ColFrags pf = M::col_frags<PSTR>(sP, lane), sf = M::col_frags<PSTR>(sS, lane);
+#pragma unroll
+            for (int dg = 0; dg < DG; ++dg) {
+                const M::ColFrags gf = M::col_frags<STR>(sG + 32 * dg, lane), qf = M::col_frags<STR>(sQ + 32 * dg, lane);
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    dv[kb][dg] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(gf.f[t], pf.f[t], dv[kb][dg], 0, 0, 0);
+                    dk[kb][dg] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qf.f[t], sf.f[t], dk[kb][dg], 0, 0, 0);
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        }
+        const int r = r0 + row;
+        if (r < end) {
+            const RowRef f = row_ref(p, b, kv, r);
+            T* dst = (T*)p.dq + f.row * p.ld_dq + (size_t)f.head * p.hd;
+#pragma unroll
+            for (int dg = 0; dg < DG; ++dg)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    float v[8];
+                    gather8(dq[dg], t, v);
+                    const int d = 32 * dg + 16 * t + 8 * half;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] *= p.scale;
+                    if (d < p.hd) store8(dst + d, v);
+                }
+        }
+    }
+    // ---- the four waves' sums, one 32-key block at a time: dk and dv side by side
+    float* sj = reinterpret_cast<float*>(smem);
+    constexpr int ONE = 4 * 32 * JSTR;
+#pragma unroll
+    for (int kb = 0; kb < NKB; ++kb) {
+        __syncthreads();
+#pragma unroll
+        for (int dg = 0; dg < DG; ++dg)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                f32x4 v, w;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    v[j] = dk[kb][dg][4 * u + j];
+                    w[j] = dv[kb][dg][4 * u + j];
+                }
+                float* at = sj + (wave * 32 + row) * JSTR + 32 * dg + 8 * u + 4 * half;
+                *reinterpret_cast<f32x4*>(at) = v;
+                *reinterpret_cast<f32x4*>(at + ONE) = w;
+            }
+        __syncthreads();
+        for (int i = tid; i < 2 * 32 * (HD / 8); i += 256) {
+            const int which = i / (32 * (HD / 8)), k32 = i / (HD / 8) % 32, d = i % (HD / 8) * 8, key = 32 * kb + k32;
+            if (key >= p.nk || d >= p.hd) continue;
+            const bool vis = key < len && (!mask || mask[key]);
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] += sj[which * ONE + (w * 32 + k32) * JSTR + d + j];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = vis ? (which ? v[j] : v[j] * p.scale) : 0.f;
+            const size_t krow = (size_t)b * p.nk + key;
+            if (p.ksplits > 1)
+                store8((which ? p.part_v : p.part_k) + (((size_t)split * p.B * p.nk + krow) * p.KV + kv) * p.hd + d, v);
+            else
+                store8((which ? (T*)p.dv + krow * p.ld_dv : (T*)p.dk + krow * p.ld_dk) + (size_t)kv * p.hd + d, v);
+        }
+    }
+}
+
 // out[row][d] = sum over the parts, in order; one thread per row, head and 8 columns.  grid.y: 0 = dk, 1 = dv
 template <typename T>
 __global__ void __launch_bounds__(256) xattn_sum_keys_kernel(BArgs p) {
@@ -445,6 +663,7 @@ __global__ void __launch_bounds__(256) xattn_sum_rows_kernel(BArgs p) {
 
 // ---------------------------------------------------------------------------------------- launch rules
 struct Plan {
+    int few;    // blocks of 32 keys of the one-kernel form, 0: two kernels
     bool two;   // dq: two row groups a wave
     int qsplits, qtiles, kw, ksplits, ktiles;
 };
@@ -462,6 +681,13 @@ int parts(long long blocks, long long tiles) {
 Plan plan_bwd(int B, int nq, int nk, int H, int KV, int hd, int dtype, bool ragged) {
     Plan pl = {};
     const long long R = (long long)nq * (H / KV), bk = (long long)B * KV, wide = (R + 255) / 256 * bk;
+    // one kernel where dk and dv of all keys fit a wave's registers
+    if (dtype == UWIR_BF16 && nq > 0 && nk > 0 && hd <= 64 && nk <= (hd <= 32 ? 128 : 64)) {
+        pl.few = (nk + 31) / 32;
+        pl.qsplits = 1;
+        pl.ksplits = parts(bk, (R + 127) / 128);
+        return pl;
+    }
     pl.qsplits = parts(bk * ((R + 127) / 128), (nk + 63) / 64);
     // 256 rows a block (bf16, up to 64 columns) where two such blocks a CU remain; with lengths per image, where the longest image's
     // blocks set the time, only from eight on.  4 x 64 x 64 queries over 2048 states, 8 heads of 64: 273 against 310 us; ragged and
@@ -494,7 +720,26 @@ Layout layout(const Plan& pl, int B, int nq, int nk, int H, int KV, int hd) {
     return l;
 }
 
+template <typename T> void launch_sum_keys(const BArgs& p, hipStream_t st) {
+    if (p.ksplits == 1) return;
+    const size_t n = (size_t)p.B * p.nk * p.KV * (p.hd / 8);
+    hipLaunchKernelGGL((xattn_sum_keys_kernel<T>), dim3((unsigned)ceil_div_sz(n, 256), 2), dim3(256), 0, st, p);
+}
+
 template <typename T, int HD> void launch(const BArgs& p, const Plan& pl, hipStream_t st) {
+    if constexpr (sizeof(T) == 2 && HD <= 64) {
+        if (pl.few) {
+            const dim3 grid(p.kblocks), block(256);
+            if (pl.few == 1) hipLaunchKernelGGL((xattn_short_bwd_kernel<HD, 1>), grid, block, 0, st, p);
+            if (pl.few == 2) hipLaunchKernelGGL((xattn_short_bwd_kernel<HD, 2>), grid, block, 0, st, p);
+            if constexpr (HD == 32) {
+                if (pl.few == 3) hipLaunchKernelGGL((xattn_short_bwd_kernel<HD, 3>), grid, block, 0, st, p);
+                if (pl.few == 4) hipLaunchKernelGGL((xattn_short_bwd_kernel<HD, 4>), grid, block, 0, st, p);
+            }
+            launch_sum_keys<T>(p, st);
+            return;
+        }
+    }
     if (p.nq > 0) {
         if (pl.two) {
             if constexpr (sizeof(T) == 2 && HD <= 64)
@@ -512,10 +757,7 @@ template <typename T, int HD> void launch(const BArgs& p, const Plan& pl, hipStr
             if (pl.kw == 2) hipLaunchKernelGGL((xattn_dkv_kernel<T, HD, 2>), dim3(p.kblocks), dim3(256), 0, st, p);
         }
         if (pl.kw == 4) hipLaunchKernelGGL((xattn_dkv_kernel<T, HD, 4>), dim3(p.kblocks), dim3(256), 0, st, p);
-        if (p.ksplits > 1) {
-            const size_t n = (size_t)p.B * p.nk * p.KV * (p.hd / 8);
-            hipLaunchKernelGGL((xattn_sum_keys_kernel<T>), dim3((unsigned)ceil_div_sz(n, 256), 2), dim3(256), 0, st, p);
-        }
+        launch_sum_keys<T>(p, st);
     }
 }
 
@@ -554,7 +796,7 @@ extern "C" int uwir_cross_attn_backward(const void* q, size_t ldq, const void* k
     p.ldm = ld_mask;
     p.B = B; p.nq = nq; p.nk = nk; p.H = heads; p.KV = kv_heads; p.hd = hd; p.G = heads / kv_heads; p.R = nq * p.G;
     p.qsplits = pl.qsplits; p.qtiles = pl.qtiles; p.ksplits = pl.ksplits; p.ktiles = pl.ktiles;
-    const long long qb = (long long)B * kv_heads * pl.qtiles * pl.qsplits, kb = (long long)B * kv_heads * pl.ktiles * pl.ksplits;
+    const long long qb = (long long)B * kv_heads * pl.qtiles * pl.qsplits, kb = (long long)B * kv_heads * (pl.few ? 1 : pl.ktiles) * pl.ksplits;
     UWIR_CHECK(qb < (1ll << 31) && kb < (1ll << 31), "cross_attn_backward: too many rows for one launch");
     p.qblocks = (int)qb; p.kblocks = (int)kb;
     p.c = scale * LOG2E; p.scale = scale; p.by_g = make_divisor(p.G);
