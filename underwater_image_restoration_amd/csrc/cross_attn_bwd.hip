@@ -48,7 +48,9 @@ __device__ __forceinline__ int image_len(const BArgs& p, int b) {
 }
 
 // ---------------------------------------------------------------------------------------- dq
-template <typename T, int HD, int QG>
+// EXACT_D: D from p and dP instead of dout . out.  out is rounded to bf16, and over few keys that moves dq and dk by 0.001 of their
+// norm (0.0004 over 1500), next to 0.0017 for their own rounding; a walk more over up to 256 keys is cheap.
+template <typename T, int HD, int QG, bool EXACT_D>
 __global__ void __launch_bounds__(256, QG == 2 ? 2 : 1) xattn_dq_kernel(BArgs p) {
     typedef Tile<T, HD> L;
     typedef typename L::M M;
@@ -128,68 +130,98 @@ __global__ void __launch_bounds__(256, QG == 2 ? 2 : 1) xattn_dq_kernel(BArgs p)
         D[g] = h.x + h.y;
         float l = ok ? p.lse[((size_t)b * p.H + f.head) * p.nq + (f.row - (size_t)b * p.nq)] * LOG2E : 0.f;
         l2[g] = l == -INFINITY ? 0.f : l;   // an image that shows nothing: no tile below has a visible key
-        if (ok && split == 0 && lane < 32) p.ld[(size_t)bk * p.R + r] = make_float2(l2[g], D[g]);
 #pragma unroll
         for (int dg = 0; dg < DG; ++dg) zero16(dq[g][dg]);
     }
     const float c = p.c;
     const bool idle = (qt * 4 + wave) * 32 * QG >= p.R;
 
-    unsigned long long bits = 0;
-    if (begin < end) {
-        load(begin);
-        bits = __ballot(vis);
-        store(0, bits);
-    }
-    __syncthreads();
-    int buf = 0;
-    for (int k0 = begin; k0 < end; k0 += KT, buf ^= 1) {
-        const bool more = k0 + KT < end;
-        if (more) load(k0 + KT);
-        if (bits && !idle) {
-#pragma unroll
-            for (int kb = 0; kb < KT / 32; ++kb) {
-                f32x16 s[QG], dp[QG];
-#pragma unroll
-                for (int g = 0; g < QG; ++g) {
-                    zero16(s[g]);
-                    zero16(dp[g]);
-                }
-                const int off = (32 * kb + (lane & 31)) * L::STR + (lane >> 5) * L::VEC;
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    const frag kf = *reinterpret_cast<const frag*>(&sK[buf][off + ks * M::KSTEP]);
-                    const frag vf = *reinterpret_cast<const frag*>(&sV[buf][off + ks * M::KSTEP]);
-#pragma unroll
-                    for (int g = 0; g < QG; ++g) {
-                        M::rows(s[g], kf, fq[g][ks]);
-                        M::rows(dp[g], vf, fg[g][ks]);
-                    }
-                }
-                const auto hider = M::hider(!(((unsigned)(bits >> (32 * kb)) >> (lane & 31)) & 1), lane);
-                typename M::Prob ds[QG];
-#pragma unroll
-                for (int g = 0; g < QG; ++g) {
-                    M::hide(s[g], hider, lane);
-                    float v[16];
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) v[r] = __builtin_amdgcn_exp2f(fmaf(s[g][r], c, -l2[g])) * (dp[g][r] - D[g]);
-                    ds[g] = M::pack(v);
-                }
-#pragma unroll
-                for (int dg = 0; dg < DG; ++dg) {
-                    const auto kt = M::template col_frags<L::STR>(&sK[buf][32 * kb * L::STR + 32 * dg], lane);
-#pragma unroll
-                    for (int g = 0; g < QG; ++g) M::cols(dq[g][dg], kt, ds[g]);
-                }
-            }
-        }
-        if (more) {
+    // one walk over the block's keys: unit(buf, kb, s, dp) for every 32 of them, s hidden where it has to be
+    auto walk = [&](auto unit) {
+        unsigned long long bits = 0;
+        if (begin < end) {
+            load(begin);
             bits = __ballot(vis);
-            store(buf ^ 1, bits);
+            store(0, bits);
         }
         __syncthreads();
+        int buf = 0;
+        for (int k0 = begin; k0 < end; k0 += KT, buf ^= 1) {
+            const bool more = k0 + KT < end;
+            if (more) load(k0 + KT);
+            if (bits && !idle) {
+#pragma unroll
+                for (int kb = 0; kb < KT / 32; ++kb) {
+                    f32x16 s[QG], dp[QG];
+#pragma unroll
+                    for (int g = 0; g < QG; ++g) {
+                        zero16(s[g]);
+                        zero16(dp[g]);
+                    }
+                    const int off = (32 * kb + (lane & 31)) * L::STR + (lane >> 5) * L::VEC;
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks) {
+                        const frag kf = *reinterpret_cast<const frag*>(&sK[buf][off + ks * M::KSTEP]);
+                        const frag vf = *reinterpret_cast<const frag*>(&sV[buf][off + ks * M::KSTEP]);
+#pragma unroll
+                        for (int g = 0; g < QG; ++g) {
+                            M::rows(s[g], kf, fq[g][ks]);
+                            M::rows(dp[g], vf, fg[g][ks]);
+                        }
+                    }
+                    const auto hider = M::hider(!(((unsigned)(bits >> (32 * kb)) >> (lane & 31)) & 1), lane);
+#pragma unroll
+                    for (int g = 0; g < QG; ++g) M::hide(s[g], hider, lane);
+                    unit(buf, kb, s, dp);
+                }
+            }
+            if (more) {
+                bits = __ballot(vis);
+                store(buf ^ 1, bits);
+            }
+            __syncthreads();
+        }
+    };
+    if constexpr (EXACT_D) {   // D = sum_k p dp in fp32, by a walk of its own
+        float d0[QG], d1[QG];
+#pragma unroll
+        for (int g = 0; g < QG; ++g) d0[g] = d1[g] = 0.f;
+        walk([&](int, int, const f32x16* s, const f32x16* dp) {
+#pragma unroll
+            for (int g = 0; g < QG; ++g)
+#pragma unroll
+                for (int r = 0; r < 16; r += 2) {
+                    d0[g] = fmaf(__builtin_amdgcn_exp2f(fmaf(s[g][r], c, -l2[g])), dp[g][r], d0[g]);
+                    d1[g] = fmaf(__builtin_amdgcn_exp2f(fmaf(s[g][r + 1], c, -l2[g])), dp[g][r + 1], d1[g]);
+                }
+        });
+#pragma unroll
+        for (int g = 0; g < QG; ++g) {
+            const float2 h = both_halves(d0[g] + d1[g]);
+            D[g] = h.x + h.y;
+        }
     }
+#pragma unroll
+    for (int g = 0; g < QG; ++g) {
+        const int r = row0 + 32 * g;
+        if (r < p.R && split == 0 && lane < 32) p.ld[(size_t)bk * p.R + r] = make_float2(l2[g], D[g]);
+    }
+    walk([&](int buf, int kb, const f32x16* s, const f32x16* dp) {
+        typename M::Prob ds[QG];
+#pragma unroll
+        for (int g = 0; g < QG; ++g) {
+            float v[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) v[r] = __builtin_amdgcn_exp2f(fmaf(s[g][r], c, -l2[g])) * (dp[g][r] - D[g]);
+            ds[g] = M::pack(v);
+        }
+#pragma unroll
+        for (int dg = 0; dg < DG; ++dg) {
+            const auto kt = M::template col_frags<L::STR>(&sK[buf][32 * kb * L::STR + 32 * dg], lane);
+#pragma unroll
+            for (int g = 0; g < QG; ++g) M::cols(dq[g][dg], kt, ds[g]);
+        }
+    });
 #pragma unroll
     for (int g = 0; g < QG; ++g) {
         const int r = row0 + 32 * g;
@@ -398,8 +430,8 @@ __global__ void __launch_bounds__(256) xattn_dkv_kernel(BArgs p) {
 }
 
 // ---------------------------------------------------------------------------------------- few keys: all three at once
-// Up to 32 NKB keys (captions, ViT states): K and V of a key head stay in LDS, its dk and dv in registers, and every row of q,
-// out and dout is read once.  Per unit (32 rows x 32 keys): S^T = K q^T and dP^T = V dout^T from LDS and registers, dq^T += K^T dS
+// Up to 32 NKB keys (captions, ViT states): K and V of a key head stay in LDS, its dk and dv in registers, and every row of q
+// and dout is read once.  Per unit (32 rows x 32 keys): S^T = K q^T and dP^T = V dout^T from LDS and registers, dq^T += K^T dS
 // from registers; P and dS go through a patch of LDS of the wave's own and come back transposed for dv^T += dout^T P and
 // dk^T += q^T dS.  5 products instead of 7.  The four waves' dk, dv (and the parts over blocks) are summed in order at the end.
 // Against the two kernels below it: 8 x 64 x 64 queries over 77 states, 8 heads of 32, 53 -> 33 us; over 50, 8 heads of 64, 66 -> 47 us.
@@ -427,22 +459,20 @@ __global__ void __launch_bounds__(256, 2) xattn_short_bwd_kernel(BArgs p) {
     const int steps = (p.R + 127) / 128, per = (steps + p.ksplits - 1) / p.ksplits;
     const int begin = min(p.R, split * per * 128), end = min(p.R, (split + 1) * per * 128);
 
-    frag fq[KS], fg[KS], fo[KS];
+    frag fq[KS], fg[KS];
     float l2 = 0.f;
-    auto fetch = [&](int r) {   // row r of q, dout, out and its lse; zeros behind the last row
+    auto fetch = [&](int r) {   // row r of q, dout and its lse; zeros behind the last row
         const bool ok = r < end;
         const RowRef f = row_ref(p, b, kv, ok ? r : 0);
         const T* Q = (const T*)p.q + f.row * p.ldq + (size_t)f.head * p.hd;
         const T* GO = (const T*)p.go + f.row * p.ldg + (size_t)f.head * p.hd;
-        const T* O = (const T*)p.o + f.row * p.ldo + (size_t)f.head * p.hd;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             const int d = ks * 16 + half * 8;
-            fq[ks] = fg[ks] = fo[ks] = frag{};
+            fq[ks] = fg[ks] = frag{};
             if (ok && d < p.hd) {
                 fq[ks] = *reinterpret_cast<const frag*>(Q + d);
                 fg[ks] = *reinterpret_cast<const frag*>(GO + d);
-                fo[ks] = *reinterpret_cast<const frag*>(O + d);
             }
         }
         l2 = ok ? p.lse[((size_t)b * p.H + f.head) * p.nq + (f.row - (size_t)b * p.nq)] : 0.f;
@@ -484,15 +514,9 @@ __global__ void __launch_bounds__(256, 2) xattn_short_bwd_kernel(BArgs p) {
         }
     const float c = p.c;
     for (; r0 < end; r0 += 128) {
-        // ---- this group's rows: D, q and dout into the wave's patch
+        // ---- this group's rows: q and dout into the wave's patch
         if (!AHEAD) fetch(r0 + row);
-        float dd = 0.f;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) dd = fmaf((float)fg[ks][j], (float)fo[ks][j], dd);
-        const float2 hs = both_halves(dd);
-        const float D = hs.x + hs.y, lr = l2 == -INFINITY ? 0.f : l2 * LOG2E;
+        const float lr = l2 == -INFINITY ? 0.f : l2 * LOG2E;
         frag q[KS], g[KS];
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
@@ -502,12 +526,7 @@ __global__ void __launch_bounds__(256, 2) xattn_short_bwd_kernel(BArgs p) {
             *reinterpret_cast<frag*>(sG + row * STR + ks * 16 + half * 8) = g[ks];
         }
         if (AHEAD && r0 + 128 < end) fetch(r0 + 128 + row);
-        f32x16 dq[DG];
-#pragma unroll
-        for (int dg = 0; dg < DG; ++dg) zero16(dq[dg]);
-#pragma unroll
-        for (int kb = 0; kb < NKB; ++kb) {
-            f32x16 s, dp;
+        auto products = [&](int kb, f32x16& s, f32x16& dp) {
             zero16(s);
             zero16(dp);
             const int off = (32 * kb + row) * STR + half * 8;
@@ -517,6 +536,29 @@ __global__ void __launch_bounds__(256, 2) xattn_short_bwd_kernel(BArgs p) {
                 M::rows(dp, *reinterpret_cast<const frag*>(sV + off + ks * 16), g[ks]);
             }
             M::hide(s, M::hider((hidden >> kb) & 1, lane), lane);
+        };
+        // D = sum_k p dp of the row in fp32, with all keys at hand.  dout . out would be one product, but out is rounded: over few
+        // keys that alone moved dq and dk by 0.001 of their norm, next to 0.0017 for their own rounding.
+        float D0 = 0.f, D1 = 0.f;
+#pragma unroll
+        for (int kb = 0; kb < NKB; ++kb) {
+            f32x16 s, dp;
+            products(kb, s, dp);
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) {
+                D0 = fmaf(__builtin_amdgcn_exp2f(fmaf(s[r], c, -lr)), dp[r], D0);
+                D1 = fmaf(__builtin_amdgcn_exp2f(fmaf(s[r + 1], c, -lr)), dp[r + 1], D1);
+            }
+        }
+        const float2 hs = both_halves(D0 + D1);
+        const float D = hs.x + hs.y;
+        f32x16 dq[DG];
+#pragma unroll
+        for (int dg = 0; dg < DG; ++dg) zero16(dq[dg]);
+#pragma unroll
+        for (int kb = 0; kb < NKB; ++kb) {
+            f32x16 s, dp;
+            products(kb, s, dp);
             float pr[16], ds[16];
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
@@ -664,6 +706,7 @@ __global__ void __launch_bounds__(256) xattn_sum_rows_kernel(BArgs p) {
 // ---------------------------------------------------------------------------------------- launch rules
 struct Plan {
     int few;    // blocks of 32 keys of the one-kernel form, 0: two kernels
+    bool exact; // dq: D by a walk of its own
     bool two;   // dq: two row groups a wave
     int qsplits, qtiles, kw, ksplits, ktiles;
 };
@@ -688,11 +731,12 @@ Plan plan_bwd(int B, int nq, int nk, int H, int KV, int hd, int dtype, bool ragg
         pl.ksplits = parts(bk, (R + 127) / 128);
         return pl;
     }
-    pl.qsplits = parts(bk * ((R + 127) / 128), (nk + 63) / 64);
+    pl.exact = dtype == UWIR_BF16 && nk <= 256;
+    pl.qsplits = pl.exact ? 1 : parts(bk * ((R + 127) / 128), (nk + 63) / 64);
     // 256 rows a block (bf16, up to 64 columns) where two such blocks a CU remain; with lengths per image, where the longest image's
     // blocks set the time, only from eight on.  4 x 64 x 64 queries over 2048 states, 8 heads of 64: 273 against 310 us; ragged and
     // with shared heads 248 against 241.
-    pl.two = dtype == UWIR_BF16 && hd <= 64 && R > 128 && pl.qsplits == 1 && wide >= (ragged ? 2048 : 512);
+    pl.two = dtype == UWIR_BF16 && !pl.exact && hd <= 64 && R > 128 && pl.qsplits == 1 && wide >= (ragged ? 2048 : 512);
     pl.qtiles = (int)((R + (pl.two ? 255 : 127)) / (pl.two ? 256 : 128));
     // few keys: waves beyond them take rows instead (fp32 rows of 128 columns leave no LDS for the longer row tiles)
     pl.kw = hd > 64 && dtype == UWIR_F32 ? 4 : nk <= 32 ? 1 : nk <= 64 ? 2 : 4;
@@ -741,11 +785,20 @@ template <typename T, int HD> void launch(const BArgs& p, const Plan& pl, hipStr
         }
     }
     if (p.nq > 0) {
-        if (pl.two) {
-            if constexpr (sizeof(T) == 2 && HD <= 64)
-                hipLaunchKernelGGL((xattn_dq_kernel<T, HD, 2>), dim3(p.qblocks), dim3(256), 0, st, p);
-        } else
-            hipLaunchKernelGGL((xattn_dq_kernel<T, HD, 1>), dim3(p.qblocks), dim3(256), 0, st, p);
+        const dim3 grid(p.qblocks), block(256);
+        bool done = false;
+        if constexpr (sizeof(T) == 2) {
+            if (pl.exact) {
+                hipLaunchKernelGGL((xattn_dq_kernel<T, HD, 1, true>), grid, block, 0, st, p);
+                done = true;
+            } else if constexpr (HD <= 64) {
+                if (pl.two) {
+                    hipLaunchKernelGGL((xattn_dq_kernel<T, HD, 2, false>), grid, block, 0, st, p);
+                    done = true;
+                }
+            }
+        }
+        if (!done) hipLaunchKernelGGL((xattn_dq_kernel<T, HD, 1, false>), grid, block, 0, st, p);
         if (p.qsplits > 1) {
             const size_t n = (size_t)p.B * p.KV * p.R * (p.hd / 8);
             hipLaunchKernelGGL((xattn_sum_rows_kernel<T>), dim3((unsigned)ceil_div_sz(n, 256)), dim3(256), 0, st, p);
