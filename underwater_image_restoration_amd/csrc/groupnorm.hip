@@ -834,9 +834,9 @@ template <typename F> int with_v(int V, F f) {
     }
 }
 
-// What the second pass reads again was read by the first: where rows in and out together outgrow the memory-side cache (256 MB),
-// written rows would drive out rows still to come, so they go past it (backward over 8 x 256 x 256 x 64 fp32: 117 -> 102 us).
-bool bypass_caches(const GnArgs& p, size_t row_bytes) { return (size_t)p.B * p.n * row_bytes > ((size_t)256 << 20); }
+// What the second pass reads again was read by the first: where rows in and out together near the size of the memory-side cache (256 MB),
+// written rows would drive out rows still to come, so they go past it (16 x 256 x 256 x 64 bf16: 87 -> 74 us).
+bool bypass_caches(const GnArgs& p, size_t row_bytes) { return (size_t)p.B * p.n * row_bytes > ((size_t)192 << 20); }
 
 void stream_shape(GnArgs& p, int V, int es) {
     p.slab = slab_channels(p.C, p.cg, V, es, 128);
