@@ -406,12 +406,14 @@ __global__ void __launch_bounds__(256) xattn_join_kernel(XArgs p) {
     const size_t pr = i / cpr;
     const int d = 8 * (int)(i % cpr);
     float m = -INFINITY;
+#pragma unroll 8
     for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.part_l[s * rows + pr]);
     float l = 0.f, v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = 0.f;
     if (m > -INFINITY)
-        for (int s = 0; s < p.splits; ++s) {
+#pragma unroll 8
+        for (int s = 0; s < p.splits; ++s) {   // eight parts' loads under way at a time
             const float w = __builtin_amdgcn_exp2f(p.part_l[s * rows + pr] - m);
             const float* src = p.part_o + (s * rows + pr) * p.hd + d;
             const f32x4 a = *reinterpret_cast<const f32x4*>(src), e = *reinterpret_cast<const f32x4*>(src + 4);
@@ -458,8 +460,9 @@ Plan plan_fwd(int B, int nq, int nk, int H, int KV, int hd, int dtype) {
         pl.qtiles = (int)((R + rows - 1) / rows);
         blocks = bk * pl.qtiles;
     }
-    // few blocks: parts of the key axis until every CU has two blocks
-    long long s = blocks >= 384 ? 1 : (512 + blocks - 1) / (blocks > 0 ? blocks : 1);
+    // few blocks: parts of the key axis until every CU has two blocks (four of the row kernel, which only streams)
+    const int want = pl.row ? 1024 : 512;
+    long long s = blocks >= 384 ? 1 : (want + blocks - 1) / (blocks > 0 ? blocks : 1);
     const long long most = nk / unit;
     if (s > most) s = most;
     if (s > 64) s = 64;

@@ -668,6 +668,7 @@ __global__ void __launch_bounds__(256) xattn_sum_keys_kernel(BArgs p) {
     float v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = 0.f;
+#pragma unroll 8
     for (int s = 0; s < p.ksplits; ++s) {
         const f32x4 a = *reinterpret_cast<const f32x4*>(src + s * stride), e = *reinterpret_cast<const f32x4*>(src + s * stride + 4);
 #pragma unroll
@@ -689,6 +690,7 @@ __global__ void __launch_bounds__(256) xattn_sum_rows_kernel(BArgs p) {
     float v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = 0.f;
+#pragma unroll 8
     for (int s = 0; s < p.qsplits; ++s) {
         const float* src = p.part_q + (s * rows + pr) * p.hd + d;
         const f32x4 a = *reinterpret_cast<const f32x4*>(src), e = *reinterpret_cast<const f32x4*>(src + 4);
