@@ -31,8 +31,9 @@ extern "C" int uwir_gamma_correction(const float* x, float* out, size_t n, float
 // two rounded products and a rounded sum, as the reference's tensor expression evaluates (no contraction into an FMA)
 __global__ void __launch_bounds__(256) mix_kernel(const float* __restrict__ lo, const float* __restrict__ hi, float* __restrict__ out,
                                                   size_t n, float a_hi, float a_lo) {
+#pragma clang fp contract(off)   // (__fmul_rn and __fadd_rn are plain operators to this compiler: they may be contracted)
     for (size_t i = blockIdx.x * (size_t)256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256)
-        out[i] = fminf(fmaxf(__fadd_rn(__fmul_rn(a_hi, hi[i]), __fmul_rn(a_lo, lo[i])), 0.f), 1.f);
+        out[i] = fminf(fmaxf(a_hi * hi[i] + a_lo * lo[i], 0.f), 1.f);
 }
 
 extern "C" int uwir_lf_hf_mix(const float* low, const float* high, double alpha, float* out, size_t n, uwir_stream_t stream) {
