@@ -82,6 +82,30 @@ def test_cross_attn_backward_refuses(kw, word):
     refused(cab(**kw), "cross_attn_backward", word)
 
 
+SPLIT = dict(nq=1, nk=8192, ws=P << 9, nb=1 << 24)     # a call that needs a workspace
+
+
+@pytest.mark.parametrize("kw,words", [
+    (dict(SPLIT, ws=(P << 4) - 256), ("workspace", "out")), (dict(SPLIT, ws=P << 1), ("workspace", "k")),
+    (dict(SPLIT, lse=P << 4), ("lse", "out")), (dict(lse=(P << 4) + 64), ("lse", "out")), (dict(lse=P), ("lse", "q")),
+    (dict(SPLIT, lse=P << 9), ("workspace", "lse"))])
+def test_cross_attn_refuses_shared_memory(kw, words):
+    refused(ca(**kw), "overlaps", *words)
+
+
+@pytest.mark.parametrize("kw,words", [
+    (dict(ws=P << 4), ("workspace", "dout")), (dict(ws=P << 6), ("workspace", "dk")), (dict(ws=(P << 5) + 16), ("workspace", "dq")),
+    (dict(lse=P << 7), ("lse", "dv")), (dict(lse=P << 8), ("workspace", "lse"))])
+def test_cross_attn_backward_refuses_shared_memory(kw, words):
+    refused(cab(**kw), "overlaps", *words)
+
+
+def test_too_many_blocks_for_a_launch():
+    Q = 1 << 40     # 64 GB of rows each
+    refused(ca(B=1024, KV=32, H=32, hd=8, nq=1 << 17, nk=1, ldq=256, ldk=256, ldv=256, ldo=256, q=Q, k=2 * Q, v=3 * Q, out=4 * Q),
+            "too many rows")
+
+
 def test_nothing_to_do_is_no_error():
     assert ca(nq=0, q=None, out=None) == 0
     assert cab(nq=0, nk=0) == 0

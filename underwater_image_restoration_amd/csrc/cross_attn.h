@@ -253,4 +253,18 @@ inline int xattn_check_mats(const char* what, int dtype, int hd, const XMat* in,
     return UWIR_OK;
 }
 
+// Memory that a call writes beside its matrices (workspace, lse) must not meet any of them.
+inline int xattn_check_apart(const char* what, const char* name, const void* p, size_t n, int dtype, int hd, const XMat* m, int count) {
+    const size_t es = dtype == UWIR_BF16 ? 2 : 4;
+    const uintptr_t x = (uintptr_t)p;
+    if (p && n)
+        for (int i = 0; i < count; ++i) {
+            if (!m[i].rows) continue;
+            const uintptr_t y = (uintptr_t)m[i].p;
+            const size_t nb = ((m[i].rows - 1) * m[i].ld + (size_t)m[i].heads * hd) * es;
+            UWIR_CHECK(x + n <= y || y + nb <= x, "%s: %s overlaps %s", what, name, m[i].name);
+        }
+    return UWIR_OK;
+}
+
 }  // namespace

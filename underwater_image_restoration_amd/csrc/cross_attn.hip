@@ -9,6 +9,8 @@
 // Either may split the key axis over blocks when there are few rows; a second launch joins the parts.
 #include "cross_attn.h"
 
+#include <utility>
+
 using namespace xattn;
 
 namespace {
@@ -509,6 +511,13 @@ extern "C" int uwir_cross_attn(const void* q, size_t ldq, const void* k, size_t 
     const size_t need = uwir_cross_attn_workspace_bytes(B, nq, nk, heads, kv_heads, hd, dtype);
     UWIR_CHECK(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
                "cross_attn: workspace too small or not 16-byte aligned");
+    const size_t nl = (size_t)B * heads * nq * sizeof(float);
+    for (const auto& m : {std::make_pair(in, 3), std::make_pair(res, 1)}) {
+        if (int rc = xattn_check_apart("cross_attn", "the workspace", workspace, need, dtype, hd, m.first, m.second)) return rc;
+        if (int rc = xattn_check_apart("cross_attn", "lse", lse, nl, dtype, hd, m.first, m.second)) return rc;
+    }
+    const uintptr_t w = (uintptr_t)workspace, l = (uintptr_t)lse;
+    UWIR_CHECK(!need || !lse || w + need <= l || l + nl <= w, "cross_attn: the workspace overlaps lse");
     const Plan pl = plan_fwd(B, nq, nk, heads, kv_heads, hd, dtype);
     XArgs p = {};
     p.q = q; p.k = k; p.v = v; p.o = out; p.lse = lse; p.lens = key_lens; p.mask = key_mask;
@@ -516,7 +525,7 @@ extern "C" int uwir_cross_attn(const void* q, size_t ldq, const void* k, size_t 
     p.B = B; p.nq = nq; p.nk = nk; p.H = heads; p.KV = kv_heads; p.hd = hd;
     p.G = heads / kv_heads; p.R = nq * p.G; p.splits = pl.splits; p.qtiles = pl.qtiles;
     const long long nb = (long long)B * kv_heads * pl.qtiles * pl.splits;
-    UWIR_CHECK(nb < (1ll << 31), "cross_attn: too many rows for one launch");
+    UWIR_CHECK(nb < (1ll << 24), "cross_attn: too many rows for one launch");   // 2^32 threads
     p.nblocks = (int)nb;
     p.c = scale * LOG2E;
     p.by_g = make_divisor(p.G);

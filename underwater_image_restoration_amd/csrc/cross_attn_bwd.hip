@@ -842,6 +842,11 @@ extern "C" int uwir_cross_attn_backward(const void* q, size_t ldq, const void* k
     const size_t need = uwir_cross_attn_backward_workspace_bytes(B, nq, nk, heads, kv_heads, hd, dtype);
     UWIR_CHECK(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
                "cross_attn_backward: workspace too small or not 16-byte aligned");
+    if (int rc = xattn_check_apart("cross_attn_backward", "the workspace", workspace, need, dtype, hd, in, 5)) return rc;
+    if (int rc = xattn_check_apart("cross_attn_backward", "the workspace", workspace, need, dtype, hd, res, 3)) return rc;
+    if (int rc = xattn_check_apart("cross_attn_backward", "lse", lse, (size_t)B * heads * nq * sizeof(float), dtype, hd, res, 3)) return rc;
+    const uintptr_t w = (uintptr_t)workspace, ls = (uintptr_t)lse;
+    UWIR_CHECK(!nq || w + need <= ls || ls + (size_t)B * heads * nq * sizeof(float) <= w, "cross_attn_backward: the workspace overlaps lse");
     const Plan pl = plan_bwd(B, nq, nk, heads, kv_heads, hd, dtype, key_lens != nullptr);
     const Layout lo = layout(pl, B, nq, nk, heads, kv_heads, hd);
     BArgs p = {};
@@ -852,7 +857,7 @@ extern "C" int uwir_cross_attn_backward(const void* q, size_t ldq, const void* k
     p.B = B; p.nq = nq; p.nk = nk; p.H = heads; p.KV = kv_heads; p.hd = hd; p.G = heads / kv_heads; p.R = nq * p.G;
     p.qsplits = pl.qsplits; p.qtiles = pl.qtiles; p.ksplits = pl.ksplits; p.ktiles = pl.ktiles;
     const long long qb = (long long)B * kv_heads * pl.qtiles * pl.qsplits, kb = (long long)B * kv_heads * (pl.few ? 1 : pl.ktiles) * pl.ksplits;
-    UWIR_CHECK(qb < (1ll << 31) && kb < (1ll << 31), "cross_attn_backward: too many rows for one launch");
+    UWIR_CHECK(qb < (1ll << 24) && kb < (1ll << 24), "cross_attn_backward: too many rows for one launch");   // 2^32 threads
     p.qblocks = (int)qb; p.kblocks = (int)kb;
     p.c = scale * LOG2E; p.scale = scale; p.by_g = make_divisor(p.G);
     char* ws = (char*)workspace;
