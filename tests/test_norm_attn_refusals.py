@@ -82,6 +82,28 @@ def test_cross_attn_backward_refuses(kw, word):
     refused(cab(**kw), "cross_attn_backward", word)
 
 
+# operands apart from each other: what a call that is not refused would look like
+GN_APART = dict(gamma=P << 6, beta=P << 7, ws=P << 8, out=P << 4)
+GNB_APART = dict(GN_APART, dy=P, x=P << 3, dx=P << 4, mean=P << 9, rstd=P << 10, dg=P << 11, db=P << 12)
+del GNB_APART["out"]
+
+
+@pytest.mark.parametrize("kw,words", [
+    (dict(mean=P << 9, rstd=P << 9), ("mean", "rstd")), (dict(mean=P << 6), ("mean", "gamma")), (dict(rstd=P << 8), ("workspace", "rstd")),
+    (dict(ws=P << 7), ("workspace", "beta")), (dict(out=(P << 6) - 256), ("out", "gamma")), (dict(ss=P << 4, ld_ss=128), ("out", "scale_shift")),
+    (dict(mean=P), ("mean", "x"))])
+def test_group_norm_act_refuses_shared_memory(kw, words):
+    refused(gn(**dict(GN_APART, **kw)), "overlaps", *words)
+
+
+@pytest.mark.parametrize("kw,words", [
+    (dict(db=P << 11), ("dgamma", "dbeta")), (dict(dg=P << 6), ("dgamma", "gamma")), (dict(db=(P << 7) + 128), ("dbeta", "beta")),
+    (dict(ss=P << 13, ld_ss=128, dss=P << 13, ld_dss=128), ("dscale_shift", "scale_shift")), (dict(ws=P << 9), ("workspace", "mean")),
+    (dict(dg=P << 3), ("dgamma", "x")), (dict(rstd=(P << 4) + 512), ("dx", "rstd")), (dict(dg=P), ("dgamma", "dy"))])
+def test_group_norm_act_backward_refuses_shared_memory(kw, words):
+    refused(gnb(**dict(GNB_APART, **kw)), "overlaps", *words)
+
+
 SPLIT = dict(nq=1, nk=8192, ws=P << 9, nb=1 << 24)     # a call that needs a workspace
 
 

@@ -920,6 +920,23 @@ bool rows_ok(const void* in, size_t ldi, int ei, const void* out, size_t ldo, in
     return d >= wi && d + wo <= si;
 }
 
+// A range of memory that a call reads or writes beside its rows.
+struct Range {
+    const void* p;
+    size_t n;
+    const char* name;
+};
+size_t ss_bytes(size_t ld, int B, int C) { return ((size_t)(B - 1) * ld + 2 * (size_t)C) * 4; }
+
+// Vectors are read again after others have been written: none that is written may meet another operand.  First `written` of all.
+int check_apart(const char* what, const Range* all, int written, int count) {
+    for (int i = 0; i < written; ++i)
+        for (int j = i + 1; j < count; ++j)
+            UWIR_CHECK(!all[i].p || !all[j].p || !overlaps(all[i].p, all[i].n, all[j].p, all[j].n), "%s: %s overlaps %s", what,
+                       all[i].name, all[j].name);
+    return UWIR_OK;
+}
+
 int check_common(const char* what, int B, int n, int C, int G, int act, size_t workspace_bytes) {
     UWIR_CHECK(B > 0 && B <= 65534 && n > 0 && C > 0 && C <= GN_MAX_C, "%s: bad shape (0 < B <= 65534, n > 0, 0 < C <= %d)", what,
                GN_MAX_C);
@@ -956,6 +973,11 @@ extern "C" int uwir_group_norm_act(const void* x, int x_dtype, size_t ldx, int B
     UWIR_CHECK(rows_ok(x, ldx, ex, out, ldo, eo, rows, C), "group_norm_act: x and out overlap");
     UWIR_CHECK(!overlaps(workspace, workspace_bytes, out, bo) && !overlaps(workspace, workspace_bytes, x, bx),
                "group_norm_act: the workspace overlaps x or out");
+    const size_t nc = (size_t)C * 4, ng = (size_t)B * groups * 4;
+    const Range all[] = {{workspace, uwir_group_norm_act_workspace_bytes(B, n, C, groups), "the workspace"}, {mean, ng, "mean"}, {rstd, ng, "rstd"},
+                         {out, bo, "out"}, {gamma, nc, "gamma"}, {beta, nc, "beta"}, {scale_shift, ss_bytes(ld_ss, B, C), "scale_shift"}, {x, bx, "x"}};
+    if (int rc = check_apart("group_norm_act", all, 3, 8)) return rc;
+    if (int rc = check_apart("group_norm_act", all + 3, 1, 4)) return rc;
     GnArgs p = {};
     p.x = x; p.out = out; p.gamma = gamma; p.beta = beta; p.ss = scale_shift; p.mean = mean; p.rstd = rstd;
     p.part = (double2*)workspace;
@@ -1002,6 +1024,13 @@ extern "C" int uwir_group_norm_act_backward(const void* dy, size_t ldy, const vo
     UWIR_CHECK(!overlaps(workspace, workspace_bytes, dx, bo) && !overlaps(workspace, workspace_bytes, x, bx) &&
                    !overlaps(workspace, workspace_bytes, dy, by),
                "group_norm_act_backward: the workspace overlaps dy, x or dx");
+    const size_t nc = (size_t)C * 4, ng = (size_t)B * groups * 4;
+    const Range all[] = {{workspace, uwir_group_norm_act_workspace_bytes(B, n, C, groups), "the workspace"},
+                         {dgamma, nc, "dgamma"}, {dbeta, nc, "dbeta"}, {dscale_shift, ss_bytes(ld_dss, B, C), "dscale_shift"},
+                         {dx, bo, "dx"}, {gamma, nc, "gamma"}, {beta, nc, "beta"}, {mean, ng, "mean"}, {rstd, ng, "rstd"},
+                         {scale_shift, ss_bytes(ld_ss, B, C), "scale_shift"}, {x, bx, "x"}, {dy, by, "dy"}};
+    if (int rc = check_apart("group_norm_act_backward", all, 4, 12)) return rc;
+    if (int rc = check_apart("group_norm_act_backward", all + 4, 1, 6)) return rc;
     GnArgs p = {};
     p.x = x; p.dy = dy; p.out = dx; p.gamma = gamma; p.beta = beta; p.ss = scale_shift; p.mean_in = mean; p.rstd_in = rstd;
     p.dgamma = dgamma; p.dbeta = dbeta; p.dss = dscale_shift;
