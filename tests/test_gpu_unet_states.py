@@ -89,3 +89,12 @@ def test_refusals():
                 dict(image_context=ctx.cuda(), context_lens=lens.cpu()), dict(image_context=ctx[:, :0].cuda())):
         with pytest.raises(ValueError):
             call(**bad)
+
+
+def test_states_of_the_host_are_refused():
+    """Kernels follow raw addresses: states (and their counts) left on the host must not reach one."""
+    _, net, xt, mu, text, ctx = setup("fp32", 5)
+    lens = torch.tensor([1, 2], dtype=torch.int32)
+    for kw in (dict(image_context=ctx), dict(image_context=ctx, context_lens=lens)):
+        with pytest.raises(ValueError, match="image_context is on cpu"):
+            net(xt.cuda(), mu.cuda(), 1, text_context=text.cuda(), **kw)

@@ -319,7 +319,8 @@ class ConditionalUNet(nn.Module):
             s1 = self._buf(tag + "s1", M, dim, f32, dev)
             ops.conv_gemm(att, a["w_o1"], s1, B=B, H=H, W=W, C_=dim, N=dim, bias=a["b_o1"], res=t0)
             ops.ln_rows(s1, a["n2"][0], a["n2"][1], h, 1e-5)
-            q2, kv2 = self._buf(tag + "q2", M, dim, adt, dev), self._buf(tag + "kv2", B * L, 2 * dim, adt, dev)
+            q2 = self._buf(tag + "q2", M, dim, adt, dev)
+            kv2 = self._buf(tag + "kv2", -(-B * L // 256) * 256, 2 * dim, adt, dev)[:B * L]   # one buffer for many lengths
             ops.gemm(h, a["w_q2"], q2)
             ops.gemm(rows, a["w_kv2"], kv2)
             nb = ops.cross_attn_workspace_bytes(B, n, L, heads, heads, 32, adt)
@@ -375,14 +376,16 @@ class ConditionalUNet(nn.Module):
         ss_all, u_all, _ = self._conditioning_rows(emb, B, B, text_context, image_context, dev, "")
         return ss_all, u_all
 
-    def _states(self, image_context, context_lens, B: int):
+    def _states(self, image_context, context_lens, B: int, dev):
         """An (B, L, context_dim) context as (rows in the GEMMs' operand type, L, lens); None for the reference's (B, context_dim)."""
-        if image_context is None or image_context.dim() == 2:
+        if image_context is None or image_context.dim() == 2 or not self._has_st:
             if context_lens is not None:
                 raise ValueError("context_lens goes with an image_context of states, (B, L, context_dim)")
             return None
         if image_context.dim() != 3 or image_context.shape[0] != B or image_context.shape[2] != self.context_dim or not image_context.shape[1]:
             raise ValueError(f"image_context must be (B, {self.context_dim}) or (B, L, {self.context_dim})")
+        if image_context.device != dev:
+            raise ValueError(f"image_context is on {image_context.device}, the image on {dev}")
         if self.context_dim % 8:
             raise ValueError("an image_context of states needs context_dim % 8 == 0")
         if context_lens is not None and (context_lens.dtype != torch.int32 or tuple(context_lens.shape) != (B,)
@@ -446,7 +449,7 @@ class ConditionalUNet(nn.Module):
         nf, td, lv, D = self.nf, 4 * self.nf, self._levels(), self.depth
         xt, cond = xt.contiguous().float(), cond.contiguous().float()
 
-        states = self._states(image_context, context_lens, B)
+        states = self._states(image_context, context_lens, B, dev)
 
         # ---- time / prompt embedding -> SiLU(t) -> all ResBlock (scale+1 | shift) vectors in one linear (or this
         # step's rows of a schedule computed once for the whole sampling loop: conditioning_schedule)
