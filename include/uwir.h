@@ -52,7 +52,7 @@ int uwir_gemm_wide_probe(const void* A, const void* Wt, void* out, const float* 
  * kernel (0 = chosen from the grid size, the default).  Results are identical for every value. */
 void uwir_dwconv_tiles_per_block(int nt);
 /* Measurement switch, no counterpart in the reference: where the packed-stream attention kernel sums its softmax
- * denominators when the V^T tile has no spare row (-1 = per-shape default, 0 = ones-operand MFMA, 1 = packed fp32 adds). */
+ * denominators when the V^T tile has no spare row (-1 = per-shape default, 0 = ones-operand MFMA, 1 = pairs of fp32 adds). */
 void uwir_attn_variant(int lsv);
 /* Measurement switch, no counterpart in the reference: bit 0 clear keeps the student's head conv on bf16 rows on the
  * per-pixel tile kernel, bit 1 set keeps its stem conv into bf16 rows on the thread-per-pixel kernel; 1 (default) takes the
@@ -286,12 +286,14 @@ int uwir_group_norm_act_backward(const void* dy, size_t ldy, const void* x, size
  * h / (heads / kv_heads) (kv_heads | heads).  A key of image b is visible if its index is below key_lens[b] (int32 [B]
  * or NULL: nk; values are clamped to [0, nk]) and key_mask[b, index] != 0 (bytes [B, ld_mask >= nk] or NULL: all):
  *   out = softmax_{visible}(scale q k^T) v [B*nq, ldo],   lse [B, heads, nq] fp32 = log sum_{visible} exp(scale q k) (may be NULL)
- * An image that shows no key gives out = 0, lse = -inf and zero gradients.  k and v of an invisible key are never used,
+ * An image that shows no key gives out = 0, lse = -inf and zero gradients.  What is visible has to be finite, scores included (a row
+ * that meets a NaN or an infinity is unspecified, other rows are not touched by a bad query).  k and v of an invisible key are never used,
  * whatever they hold; their gradients are written as zeros.  backward: dq, dk, dv (written, not added to) from out, lse of
- * the forward call and dout; the gradients of shared key heads are summed over their query heads in a fixed order.
+ * the forward call and dout (sum_d dout out is formed from p and dout v^T instead where bf16 keys are at most 256); the gradients of shared key heads are summed over their query heads in a fixed order.
  * All tensors of a call share a dtype (fp32: exact-fp32 MFMA; bf16: bf16 MFMA operands with probabilities and score
  * gradients rounded to bf16, fp32 accumulation and statistics).  hd % 8 == 0, hd <= 128; rows and strides 16-byte aligned;
- * 1e-20 <= scale <= 1e20; row strides below 32 MB; nq, nk >= 0; B * kv_heads <= 65535.  Outputs must not overlap any other operand.
+ * 1e-20 <= scale <= 1e20; row strides below 32 MB; nq, nk >= 0; B * kv_heads <= 65535.  Outputs, lse and the workspace must not share memory with another operand (column ranges of one
+ * wider matrix that do not meet are fine).
  * workspace: >= the matching *_workspace_bytes (may be 0), 16-byte aligned; calls that may run at the same
  * time need one each (captured graphs included).  Results do not depend on scheduling. */
 size_t uwir_cross_attn_workspace_bytes(int B, int nq, int nk, int heads, int kv_heads, int hd, int dtype);

@@ -642,7 +642,7 @@ __global__ void __launch_bounds__(256) attn_pack_kernel(const bf16_t* __restrict
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 // Denominators when the V^T tile has no spare row for a ones row (LSV): 0 = a ones-operand 32x32x16 MFMA per 16 keys
-// (every one of its 32 output rows is the same sum: 64 MFMA cycles per 32 x 32 block); 1 = packed fp32 adds of the
+// (every one of its 32 output rows is the same sum: 64 MFMA cycles per 32 x 32 block); 1 = fp32 adds of the
 // exponentials on the VALU (8 per block, on the pipe that bounds this kernel); 2 = a 16x16x32 MFMA whose A operand is
 // a 0/1 selector: fed the 32x32x16 B fragment as it is, lane group G of its k dimension holds queries 16 (G & 1) + n,
 // key half G >> 1, so row 0 = groups {0, 2} and row 1 = groups {1, 3} give the sums of queries n and n + 16: half the

@@ -1,9 +1,10 @@
 // Cross attention, backward.  With s = scale q k^T over the visible keys and p = exp(s - lse):
 //   D = sum_d dout out,  dv = p^T dout,  dp = dout v^T,  ds = p (dp - D),  dq = scale ds k,  dk = scale ds^T q
-// More than a few keys take two kernels, each of which keeps its result in registers and forms p again (7 products instead of the 5 that one kernel
-// with both results would need; in exchange nothing is accumulated through memory in an order that changes):
+// More than a few keys take two kernels, each of which keeps its result in registers and forms p again (7 products instead of
+// the 5 that one kernel with both results would need; in exchange nothing is accumulated through memory in an order that
+// changes):
 //   rows kernel  a wave owns 32 packed rows (cross_attn.hip), walks the keys: S^T = K q^T, dP^T = V dout^T,
-//                dq^T += K^T dS; also forms D and hands (lse, D) to the next kernel in packed-row order
+//                dq^T += K^T dS; also forms D (few bf16 keys: from p and dP) and hands (lse, D) to the next kernel in packed-row order
 //   keys kernel  a wave owns 32 keys, walks the rows of all query heads that share them: S = q K^T, dP = dout V^T,
 //                dv^T += dout^T P, dk^T += q^T dS -- the sum over shared heads and rows never leaves the registers
 // Either splits its long axis over blocks when there are few; the parts (fp32) are then summed in order by a last launch.
@@ -50,6 +51,8 @@ __device__ __forceinline__ int image_len(const BArgs& p, int b) {
 // ---------------------------------------------------------------------------------------- dq
 // EXACT_D: D from p and dP instead of dout . out.  out is rounded to bf16, and over few keys that moves dq and dk by 0.001 of their
 // norm (0.0004 over 1500), next to 0.0017 for their own rounding; a walk more over up to 256 keys is cheap.
+// Bound by vector issue as the forward kernel is, with two products in and one out a unit: 4 x 64 x 64 queries over up to 2048 states of
+// lengths of their own, 8 heads of 64 on 2 key heads, 100 us.
 template <typename T, int HD, int QG, bool EXACT_D>
 __global__ void __launch_bounds__(256, QG == 2 ? 2 : 1) xattn_dq_kernel(BArgs p) {
     typedef Tile<T, HD> L;
@@ -247,6 +250,8 @@ __global__ void __launch_bounds__(256, QG == 2 ? 2 : 1) xattn_dq_kernel(BArgs p)
 }
 
 // ---------------------------------------------------------------------------------------- dk, dv
+// Bound by vector issue too: four products a unit, P and dS rounded in between, lse and D of every row read from LDS.  The same case
+// takes 140 us (410 TF of 10 hd flops a pair together with the rows kernel; 600-630 over images of one length).
 // KW waves across the keys (32 each); the 4 / KW waves of one key group take the 32-row blocks of a tile in turn
 template <typename T, int HD, int KW>
 __global__ void __launch_bounds__(256) xattn_dkv_kernel(BArgs p) {
