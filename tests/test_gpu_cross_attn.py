@@ -157,6 +157,18 @@ def test_many_rows(ops, dt):
         check(ops, inputs(*dims, "both", dt, seed=4), dims, grads=False)
 
 
+@pytest.mark.parametrize("keys", ["none", "mask"])
+@pytest.mark.parametrize("dims", [(16, 2053, 1, 8, 8, 32), (16, 2053, 64, 8, 8, 32), (16, 2053, 300, 8, 8, 24), (8, 4800, 65, 8, 8, 64),
+                                  (8, 1203, 577, 32, 8, 64), (16, 2100, 130, 8, 8, 56)], ids=lambda d: "x".join(map(str, d)))
+def test_wide_row_tiles(ops, dims, keys):
+    """Many row tiles over one, some and many tiles of keys, a ragged last one, shared heads, heads narrower than the kernel's, an image
+    that shows nothing; the same answer every time."""
+    t = inputs(*dims, keys, BF, seed=3)
+    check(ops, t, dims, grads=False)
+    first = forward(ops, t, *dims)
+    assert all(torch.equal(a, b) for _ in range(3) for a, b in zip(first, forward(ops, t, *dims)))
+
+
 @pytest.mark.parametrize("dt", [BF, F32], ids=["bf16", "f32"])
 @pytest.mark.parametrize("dims", [(3, 40, 150, 4, 2, 32), (3, 2, 150, 4, 2, 64), (3, 40, 40, 2, 2, 128)])
 def test_hidden_keys_may_hold_anything(ops, dims, dt):
