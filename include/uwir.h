@@ -266,7 +266,7 @@ int uwir_flash_attn(const void* q, int ldq, const void* k, int ldk, const void* 
  * type).  backward: dy, x, dx share a dtype; dgamma, dbeta [C] fp32 (written, not added to), dscale_shift [B, ld_dss]
  * [dscale | dshift] or NULL; dx may be dy or x itself; no other output
  * may share memory with another operand.  Statistics and sums are fp32 per thread and fp64 beyond, in a fixed order:
- * results do not depend on scheduling.  C <= 2048, B <= 65534; any C, strides and element alignment (16-byte aligned
+ * results do not depend on scheduling.  C <= 2048, B <= 65534, n < 2^30; any C, strides and element alignment (16-byte aligned
  * rows with C a multiple of 8 (bf16) or 4 (fp32) run at full width).  workspace (both directions):
  * >= uwir_group_norm_act_workspace_bytes, 16-byte aligned, contents never carried between calls; calls that may
  * run at the same time need one each (captured graphs included). */

@@ -953,8 +953,9 @@ int check_apart(const char* what, const Range* all, int written, int count) {
 }
 
 int check_common(const char* what, int B, int n, int C, int G, int act, size_t workspace_bytes) {
-    UWIR_CHECK(B > 0 && B <= 65534 && n > 0 && C > 0 && C <= GN_MAX_C, "%s: bad shape (0 < B <= 65534, n > 0, 0 < C <= %d)", what,
-               GN_MAX_C);
+    // row indexes are 32 bits, and a thread looks up to 4 rows of each of GN_T lanes ahead
+    UWIR_CHECK(B > 0 && B <= 65534 && n > 0 && n < (1 << 30) && C > 0 && C <= GN_MAX_C,
+               "%s: bad shape (0 < B <= 65534, 0 < n < 2^30, 0 < C <= %d)", what, GN_MAX_C);
     UWIR_CHECK(G > 0 && C % G == 0, "%s: groups must divide C", what);
     UWIR_CHECK(act == UWIR_ACT_NONE || act == UWIR_ACT_SILU, "%s: act must be UWIR_ACT_NONE or UWIR_ACT_SILU", what);
     UWIR_CHECK(workspace_bytes >= uwir_group_norm_act_workspace_bytes(B, n, C, G), "%s: workspace too small", what);
