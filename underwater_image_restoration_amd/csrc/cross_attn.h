@@ -111,7 +111,8 @@ __device__ __forceinline__ void zero16(f32x16& a) {
 }
 
 // A tile of rows of a matrix in global memory as a buffer: rows from `row` on, of which those below `end` exist; anything
-// beyond reads as zeros, so that neither clamps nor selects sit in the loops.  `ldb`, `width` in bytes, ldb < 2^25.
+// beyond reads as zeros, so that neither clamps nor selects sit in the loops.  `ldb`, `width` in bytes, width <= ldb; a buffer holds
+// 2^31 - 1 bytes: the rows that a block reaches in it times ldb stay below that (64 rows of ldb < 2^25).
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_buffer(const void* base, size_t ldb, int row, int end, int width) {
     const size_t bytes = row < end ? (size_t)(end - row - 1) * ldb + width : 0;
     return __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)base + (size_t)row * ldb), 0,

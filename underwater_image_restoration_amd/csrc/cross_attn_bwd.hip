@@ -281,7 +281,8 @@ __global__ void __launch_bounds__(256) xattn_dkv_kernel(BArgs p) {
     const size_t ldqb = p.ldq * sizeof(T), ldgb = p.ldg * sizeof(T);
     const T* Q = (const T*)p.q + (size_t)b * p.nq * p.ldq + (size_t)kv * p.G * p.hd;
     const T* GO = (const T*)p.go + (size_t)b * p.nq * p.ldg + (size_t)kv * p.G * p.hd;
-    // a tile's packed rows lie in the rows from the first one's query on, G heads side by side: a buffer at that query
+    // a tile's packed rows lie in the rows from the first one's query on, G heads side by side: a buffer at that query.  RT - 1 rows and
+    // one row's heads stay below 2^31 bytes: 63 x 32 MB, or 127 x 16 MB by the launch rule of kw = 1
     auto load = [&](int r0) {
         const int q0 = (int)p.by_g.quot((unsigned)r0);
         const __amdgpu_buffer_rsrc_t qb = tile_buffer(Q, ldqb, q0, p.nq, width * p.G), gb = tile_buffer(GO, ldgb, q0, p.nq, width * p.G);
@@ -728,7 +729,8 @@ int parts(long long blocks, long long tiles) {
     return s < 1 ? 1 : (int)s;
 }
 
-Plan plan_bwd(int B, int nq, int nk, int H, int KV, int hd, int dtype, bool ragged) {
+// `far`: rows of q or dout lie 16 MB apart or more
+Plan plan_bwd(int B, int nq, int nk, int H, int KV, int hd, int dtype, bool ragged, bool far) {
     Plan pl = {};
     const long long R = (long long)nq * (H / KV), bk = (long long)B * KV, wide = (R + 255) / 256 * bk;
     // one kernel where dk and dv of all keys fit a wave's registers
@@ -745,8 +747,9 @@ Plan plan_bwd(int B, int nq, int nk, int H, int KV, int hd, int dtype, bool ragg
     // with shared heads 248 against 241.
     pl.two = dtype == UWIR_BF16 && !pl.exact && hd <= 64 && R > 128 && pl.qsplits == 1 && wide >= (ragged ? 2048 : 512);
     pl.qtiles = (int)((R + (pl.two ? 255 : 127)) / (pl.two ? 256 : 128));
-    // few keys: waves beyond them take rows instead (fp32 rows of 128 columns leave no LDS for the longer row tiles)
-    pl.kw = hd > 64 && dtype == UWIR_F32 ? 4 : nk <= 32 ? 1 : nk <= 64 ? 2 : 4;
+    // few keys: waves beyond them take rows instead (fp32 rows of 128 columns leave no LDS for the longer row tiles; the 128 rows of
+    // kw = 1 have to lie within the 2^31 bytes of a buffer, those of kw = 2 are 64.  Both have the same parts for 32 keys)
+    pl.kw = hd > 64 && dtype == UWIR_F32 ? 4 : nk <= 32 && !far ? 1 : nk <= 64 ? 2 : 4;
     pl.ktiles = (nk + 32 * pl.kw - 1) / (32 * pl.kw);
     pl.ksplits = parts(bk * pl.ktiles, (R + 63) / 64);
     return pl;
@@ -825,7 +828,7 @@ template <typename T, int HD> void launch(const BArgs& p, const Plan& pl, hipStr
 
 extern "C" size_t uwir_cross_attn_backward_workspace_bytes(int B, int nq, int nk, int heads, int kv_heads, int hd, int dtype) {
     if (B <= 0 || nq < 0 || nk < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || hd <= 0) return 0;
-    return layout(plan_bwd(B, nq, nk, heads, kv_heads, hd, dtype, false), B,   // the parts do not depend on the lengths
+    return layout(plan_bwd(B, nq, nk, heads, kv_heads, hd, dtype, false, false), B,   // the parts do not depend on lengths and strides
                    nq, nk, heads, kv_heads, hd).total;
 }
 
@@ -852,7 +855,8 @@ extern "C" int uwir_cross_attn_backward(const void* q, size_t ldq, const void* k
     if (int rc = xattn_check_apart("cross_attn_backward", "lse", lse, (size_t)B * heads * nq * sizeof(float), dtype, hd, res, 3)) return rc;
     const uintptr_t w = (uintptr_t)workspace, ls = (uintptr_t)lse;
     UWIR_CHECK(!nq || w + need <= ls || ls + (size_t)B * heads * nq * sizeof(float) <= w, "cross_attn_backward: the workspace overlaps lse");
-    const Plan pl = plan_bwd(B, nq, nk, heads, kv_heads, hd, dtype, key_lens != nullptr);
+    const size_t apart = (ldq > ld_dout ? ldq : ld_dout) * (dtype == UWIR_BF16 ? 2 : 4);
+    const Plan pl = plan_bwd(B, nq, nk, heads, kv_heads, hd, dtype, key_lens != nullptr, apart >= (1u << 24));
     const Layout lo = layout(pl, B, nq, nk, heads, kv_heads, hd);
     BArgs p = {};
     p.q = q; p.k = k; p.v = v; p.o = out; p.go = dout; p.lse = lse; p.dq = dq; p.dk = dk; p.dv = dv;
