@@ -24,3 +24,57 @@ def test_rows_20_mb_apart(ops, dims, dt):
         cols.copy_(t[name])
         t[name] = cols
     check(ops, t, dims)
+
+
+def call(ops, t, dims, scale):
+    B, nq, nk, H, KV, hd = dims
+    dt = t["q"].dtype
+    nan = lambda *s, d=dt: torch.full(s, float("nan"), dtype=d, device="cuda")  # noqa: E731
+    r = dict(out=nan(B * nq, H * hd), lse=nan(B, H, nq, d=F32), dq=nan(B * nq, H * hd), dk=nan(B * nk, KV * hd), dv=nan(B * nk, KV * hd))
+    nb = max(ops.cross_attn_workspace_bytes(*dims, dt), ops.cross_attn_backward_workspace_bytes(*dims, dt))
+    ws = torch.full((nb,), 0xff, dtype=torch.uint8, device="cuda")
+    kw = dict(key_lens=t["lens"], key_mask=t["mask"])
+    ops.cross_attn(t["q"], t["k"], t["v"], *dims, scale, r["out"], ws, lse=r["lse"], **kw)
+    ops.cross_attn_backward(t["q"], t["k"], t["v"], r["out"], r["lse"], t["do"], *dims, scale, r["dq"], r["dk"], r["dv"], ws, **kw)
+    return r
+
+
+@pytest.mark.parametrize("dt", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("dims", [(2, 70, 100, 2, 2, 32), (2, 300, 400, 4, 2, 64), (1, 40, 20, 1, 1, 128), (2, 1, 400, 4, 2, 64),
+                                  (16, 2053, 100, 8, 8, 32)], ids=lambda d: "x".join(map(str, d)))
+def test_scale_of_any_size(ops, dims, dt):
+    """q and k smaller and the scale larger by the same powers of two (and the other way round): the same scores, bit for bit, with
+    units of 32 keys that the mask hides wholly at the start and beside shown ones."""
+    B, nq, nk, H, KV, hd = dims
+    t = inputs(*dims, "mask", dt, seed=nk)
+    t["mask"][:, :32] = nk <= 32
+    t["mask"][:, 64:96] = False
+    t["mask"][0, 40:] = True
+    want = call(ops, t, dims, hd ** -0.5)
+    assert all(bool(torch.isfinite(want[n]).all()) for n in ("out", "dq", "dk", "dv"))
+    for e in (17, 32, -30):     # scales 3e9 and up, 3e18 and up, 3e-19 and down
+        s = dict(t, q=t["q"] * 2.0 ** -e, k=t["k"] * 2.0 ** -e)
+        got = call(ops, s, dims, hd ** -0.5 * 4.0 ** e)
+        for n in ("out", "lse", "dv"):
+            assert torch.equal(got[n], want[n]), (n, e)
+        for n in ("dq", "dk"):
+            assert torch.equal(got[n], want[n] * 2.0 ** e), (n, e)
+
+
+@pytest.mark.parametrize("dt", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("nq", [1, 50])
+def test_scores_far_below_zero(ops, nq, dt):
+    """Every product q k is -1e31 or -2e31: the former share the row evenly, the latter get nothing.  lse = -8 2^34 + log(count): the
+    sum is lost in the product's rounding, one of fp32 for the product and one for the logarithm's base each way: 4 u of it."""
+    dims = B, nq, nk, H, KV, hd = (1, nq, 90, 2, 2, 8)
+    t = inputs(*dims, "none", dt, seed=5)
+    t["q"] = torch.full_like(t["q"], 2.0 ** 50)
+    near = torch.arange(nk, device="cuda") % 3 == 0
+    t["k"] = torch.where(near[:, None], -2.0 ** 50, -2.0 ** 51).to(dt).expand(nk, H * hd).contiguous()
+    r = call(ops, t, dims, 2.0 ** -66)
+    mean = t["v"].double()[near].mean(0)
+    # 30 equal probabilities: 1/30 formed by a reciprocal (u), sums of 30 terms, the store's half step
+    tol = 40 * U * t["v"].double()[near].abs().mean(0) + (2.0 ** -8 if dt == BF else U) * mean.abs()
+    assert bool(((r["out"].double() - mean).abs() <= tol).all())
+    lse = -8 * 2.0 ** 34 + math.log(30)
+    assert bool(((r["lse"].double() - lse).abs() <= 4 * U * abs(lse)).all())

@@ -30,6 +30,7 @@ struct XArgs {
     int B, nq, nk, H, KV, hd, G, R, splits, nblocks, qtiles;
     Divisor by_g;
     float c;            // scale * log2(e)
+    float m0;           // the running reference before any key is seen: low, and m0 * c finite
 };
 
 template <typename T, int HD> struct Tile {
@@ -70,14 +71,16 @@ template <typename T, int HD> struct Group {
         }
 #pragma unroll
         for (int g = 0; g < DG; ++g) zero16(o[g]);
-        m = -1e30f;
+        m = p.m0;
         l = 0.f;
     }
 
     // Scores s of 32 keys -> probabilities relative to the running reference m.  m need not be the maximum, only near enough for
     // the fp32 range: the probabilities are formed first, and only where a lane's sum leaves 2^64 is the true maximum taken, the
-    // output rescaled and the unit formed again (the very first unit does so by itself: m starts at -1e30).  A reference below the
-    // maximum costs no accuracy; what underflows next to it is below 2^-120 of a sum that is at least 1.
+    // output rescaled and the unit formed again.  A reference below the maximum costs no accuracy; what underflows next to it is
+    // below 2^-120 of a sum that is at least 1.  The first unit with a visible key does so by itself: m starts at m0, half the fp32
+    // range below zero in scores and in their products with c, so that visible scores lie far above it and hidden ones far below,
+    // and a unit without a visible key leaves it there, with probabilities of 0.
     static __device__ __forceinline__ bool out_of_range(float sum) { return sum > 1.8446744e19f; }
     __device__ __forceinline__ void rescale(const f32x16& s, float c, typename M::Prob& pb, float& sum) {
         float mx = fmaxf(s[0], s[1]);
@@ -383,7 +386,7 @@ __global__ void __launch_bounds__(256) xattn_row_kernel(XArgs p) {
         sl[wave][lane] = h.x + h.y;
     }
     __syncthreads();   // also: every wave is done with its tiles, smem becomes the outputs' buffer
-    float m = -1e30f, l = 0.f;
+    float m = p.m0, l = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) m = fmaxf(m, sm[w][lane & 31]);
 #pragma unroll
@@ -539,6 +542,7 @@ extern "C" int uwir_cross_attn(const void* q, size_t ldq, const void* k, size_t 
     UWIR_CHECK(nb < (1ll << 24), "cross_attn: too many rows for one launch");   // 2^32 threads
     p.nblocks = (int)nb;
     p.c = scale * LOG2E;
+    p.m0 = p.c > 1.f ? -1.7e38f / p.c : -1.7e38f;
     p.by_g = make_divisor(p.G);
     if (need) {
         p.part_o = (float*)workspace;
