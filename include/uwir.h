@@ -286,8 +286,9 @@ int uwir_group_norm_act_backward(const void* dy, size_t ldy, const void* x, size
  * h / (heads / kv_heads) (kv_heads | heads).  A key of image b is visible if its index is below key_lens[b] (int32 [B]
  * or NULL: nk; values are clamped to [0, nk]) and key_mask[b, index] != 0 (bytes [B, ld_mask >= nk] or NULL: all):
  *   out = softmax_{visible}(scale q k^T) v [B*nq, ldo],   lse [B, heads, nq] fp32 = log sum_{visible} exp(scale q k) (may be NULL)
- * An image that shows no key gives out = 0, lse = -inf and zero gradients.  What is visible has to be finite, scores included, q k and scale q k each within +-1e38 (a row
- * that meets a NaN or an infinity is unspecified, other rows are not touched by a bad query).  k and v of an invisible key are never used,
+ * An image that shows no key gives out = 0, lse = -inf and zero gradients.  What is visible has to be finite, q k and
+ * scale q k each within +-1e38, nk max |v| below 8e34 (a row that meets a NaN or an infinity is unspecified, other rows
+ * are not touched by a bad query).  k and v of an invisible key are never used,
  * whatever they hold; their gradients are written as zeros.  backward: dq, dk, dv (written, not added to) from out, lse of
  * the forward call and dout (sum_d dout out is formed from p and dout v^T instead where bf16 keys are at most 256); the gradients of shared key heads are summed over their query heads in a fixed order.
  * All tensors of a call share a dtype (fp32: exact-fp32 MFMA; bf16: bf16 MFMA operands with probabilities and score

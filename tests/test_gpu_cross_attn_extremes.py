@@ -78,3 +78,17 @@ def test_scores_far_below_zero(ops, nq, dt):
     assert bool(((r["out"].double() - mean).abs() <= tol).all())
     lse = -8 * 2.0 ** 34 + math.log(30)
     assert bool(((r["lse"].double() - lse).abs() <= 4 * U * abs(lse)).all())
+
+
+@pytest.mark.parametrize("dt", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("dims", [(2, 70, 300, 2, 2, 16), (2, 2, 300, 2, 2, 16), (16, 2053, 300, 8, 8, 16)], ids=lambda d: "x".join(map(str, d)))
+def test_large_values_under_rising_scores(ops, dims, dt):
+    """v of 1e22 beside scores that rise from 0 to 40 along the keys: e^40 1e22 would pass the fp32 range, the answer does not."""
+    B, nq, nk, H, KV, hd = dims
+    t = inputs(*dims, "none", dt, seed=7)
+    q, k = torch.zeros(B * nq, H, hd, device="cuda"), torch.zeros(B, nk, KV, hd, device="cuda")
+    q[..., 0] = 4        # scale 1/4
+    k[:, 128:, :, 0] = 40
+    t["q"], t["k"] = q.reshape(B * nq, -1).to(dt), k.reshape(B * nk, -1).to(dt)
+    t["v"] = (t["v"].float() * 1e22).to(dt)
+    check(ops, t, dims, grads=nq < 100)

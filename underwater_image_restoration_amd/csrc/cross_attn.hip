@@ -7,9 +7,9 @@
 //   tile kernel   4 waves x 32 QG rows share key tiles in LDS
 //   row kernel    R <= 32: the 4 waves take key tiles of their own and join at the end
 // Either may split the key axis over blocks when there are few rows; a second launch joins the parts.
-// The running maximum is only raised when a lane's sum passes 2^64: until then the probabilities of the maximum held are exact enough
-// (fp32 keeps its 24 bits at any exponent), and the usual tile pays no rescale.  Probabilities are rounded to bf16 for the second
-// product (2^-9 of each at most), their sum is that of the unrounded ones.
+// The running maximum is only raised when a lane's sum over a unit passes 2^16: until then the probabilities of the maximum held
+// are exact enough (fp32 keeps its 24 bits at any exponent), and the usual tile pays no rescale.  Probabilities are rounded to bf16
+// for the second product (2^-8 of each at most), their sum is that of the unrounded ones.
 #include "cross_attn.h"
 
 #include <utility>
@@ -76,12 +76,13 @@ template <typename T, int HD> struct Group {
     }
 
     // Scores s of 32 keys -> probabilities relative to the running reference m.  m need not be the maximum, only near enough for
-    // the fp32 range: the probabilities are formed first, and only where a lane's sum leaves 2^64 is the true maximum taken, the
+    // the fp32 range: the probabilities are formed first, and only where a lane's sum leaves 2^16 is the true maximum taken, the
     // output rescaled and the unit formed again.  A reference below the maximum costs no accuracy; what underflows next to it is
-    // below 2^-120 of a sum that is at least 1.  The first unit with a visible key does so by itself: m starts at m0, half the fp32
-    // range below zero in scores and in their products with c, so that visible scores lie far above it and hidden ones far below,
-    // and a unit without a visible key leaves it there, with probabilities of 0.
-    static __device__ __forceinline__ bool out_of_range(float sum) { return sum > 1.8446744e19f; }
+    // below 2^-120 of a sum that is at least 1; and the output before its division stays below nk 2^12 max |v|.
+    // The first unit with a visible key does so by itself: m starts at m0, half the fp32 range below zero in scores and in their
+    // products with c, so that visible scores lie far above it and hidden ones far below, and a unit without a visible key leaves
+    // it there, with probabilities of 0.
+    static __device__ __forceinline__ bool out_of_range(float sum) { return sum > 65536.f; }
     __device__ __forceinline__ void rescale(const f32x16& s, float c, typename M::Prob& pb, float& sum) {
         float mx = fmaxf(s[0], s[1]);
 #pragma unroll
