@@ -262,7 +262,8 @@ int uwir_flash_attn(const void* q, int ldq, const void* k, int ldk, const void* 
  *   xh = (x - mean) rstd,  rstd = 1 / sqrt(var + eps)            var biased, as nn.GroupNorm
  *   z  = (xh gamma + beta) (1 + scale_b) + shift_b               scale_shift [B, ld_ss] = [scale (C) | shift (C)] or NULL
  *   out = act(z)                                                 UWIR_ACT_NONE or UWIR_ACT_SILU; fp32 or bf16 rows
- * mean, rstd [B, G] fp32 (each may be NULL) are what the backward pass wants kept.  out may be x itself (same stride and
+ * Values up to 1e37 whose distances to their group's mean stay below 6e18 / sqrt(n) are in range; an infinity or a NaN makes its
+ * group NaN.  mean, rstd [B, G] fp32 (each may be NULL) are what the backward pass wants kept.  out may be x itself (same stride and
  * type).  backward: dy, x, dx share a dtype; dgamma, dbeta [C] fp32 (written, not added to), dscale_shift [B, ld_dss]
  * [dscale | dshift] or NULL; dx may be dy or x itself; no other output
  * may share memory with another operand.  Statistics and sums are fp32 per thread and fp64 beyond, in a fixed order:

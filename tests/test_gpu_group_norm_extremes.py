@@ -1,0 +1,54 @@
+"""GPU: group_norm_act on values that leave the range of squares, on infinities and NaN, and on rows so many that one thread takes
+thousands.  Tolerances are those of test_gpu_group_norm_act.py."""
+import pytest
+import torch
+
+from tests.test_gpu_group_norm_act import EPS, HALF, U, close, make, ops, reference  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def forward(ops, x, gamma, beta, B, n, C, G, act=0, ss=None):
+    y, mean, rstd = torch.full_like(x, float("nan")), torch.empty(B, G, device="cuda"), torch.empty(B, G, device="cuda")
+    ws = torch.empty(ops.group_norm_act_workspace_bytes(B, n, C, G), dtype=torch.uint8, device="cuda")
+    ops.group_norm_act(x, B, n, C, G, EPS, gamma, beta, y, ws, act=act, scale_shift=ss, mean=mean, rstd=rstd)
+    return y, mean, rstd, ws
+
+
+# one launch and two, one element a vector and many, one group wider than a block
+SHAPES = [(1, 64, 64, 8), (2, 33, 15, 5), (2, 5000, 64, 8), (2, 3000, 30, 3), (1, 700, 2047, 1)]
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("B,n,C,G", SHAPES)
+def test_mean_whose_square_leaves_the_range(ops, B, n, C, G, dt):
+    """Values of 3e19 (1 +- 1e-2): the mean's square is past fp32, the variance is not.  rstd: a thread's mean of up to 8 rows is a sum
+    and a product in fp32, off by d <= 8 u |m|; the variance is that of the threads' means as they are held, plus the squares about
+    them, so it is off by 2 cov(means, d) <= 2 sigma d: 16 u |m| / sigma of itself, rstd by half of that.  (|m| / sigma is 150
+    here, not the 1 for which 8 u hold.)"""
+    x, gamma, beta, _, _ = make(B, n, C, False, torch.float32, seed=n)
+    x = (3e19 * (1 + 0.01 * torch.tanh(x))).to(dt)
+    y, mean, rstd, _ = forward(ops, x, gamma, beta, B, n, C, G)
+    r = reference(x, gamma, beta, None, B, n, C, G, False)
+    close(y, r["y"], r["ty"], HALF[dt])
+    close(mean, r["mean"], 4 * U * x.double().abs().max(), U)
+    close(rstd, r["rstd"], 8 * U * r["rstd"] * (1 + r["mean"].abs() * r["rstd"]), U)
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("B,n,C,G", SHAPES)
+def test_a_diverged_group_shows(ops, B, n, C, G, dt, bad):
+    """One infinity or NaN makes its own group NaN, statistics included, and leaves the others as they were."""
+    x, gamma, beta, _, _ = make(B, n, C, False, dt, seed=n)
+    want, wm, wr, _ = forward(ops, x, gamma, beta, B, n, C, G)
+    hit = x.clone()
+    hit[n - 1, C - 1] = bad     # the last group of the first image
+    y, mean, rstd, _ = forward(ops, hit, gamma, beta, B, n, C, G)
+    assert bool(torch.isnan(rstd[0, -1])) and not bool(torch.isfinite(mean[0, -1]))
+    group = torch.zeros(B * n, C, dtype=torch.bool, device="cuda")
+    group[:n, C - C // G:] = True
+    assert bool(torch.isnan(y[group]).all()) and torch.equal(y[~group], want[~group])
+    stats = torch.zeros(B, G, dtype=torch.bool, device="cuda")
+    stats[0, -1] = True
+    assert torch.equal(mean[~stats], wm[~stats]) and torch.equal(rstd[~stats], wr[~stats])

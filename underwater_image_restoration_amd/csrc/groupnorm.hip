@@ -8,7 +8,8 @@
 //   streamed  a chunk of rows: statistics in one launch, output in the next; the second read of x comes from the L2 (the
 //             same block index runs on the same XCD) or the memory-side cache where the map fits
 // Statistics: every thread reduces batches of rows to (mean, sum of squared distances to that mean) per channel and
-// merges them pairwise, so that a mean far from zero or a stray first element costs no digits; everything across
+// merges them pairwise, so that a stray first element costs no digits and a mean far from zero costs the variance |mean| / sigma
+// roundings, not the square of that; everything across
 // threads is summed in fp64 in a fixed order (results do not depend on scheduling).
 #include "common.h"
 #include <type_traits>
@@ -86,7 +87,7 @@ template <int V> struct Stat {
             }
             const float d = m - mean[j];
             mean[j] = fmaf(d, wa, mean[j]);
-            m2[j] += fmaf(d * d, wb, q);
+            m2[j] += cnt ? fmaf(d * d, wb, q) : q;   // of the first batch d is the mean itself: its square may leave the range
         }
         cnt += k;
     }
@@ -249,8 +250,8 @@ __device__ __forceinline__ void slab_group_sums(const GnArgs& p, const Place& l,
 
 __device__ __forceinline__ float2 finish_stats(double s, double q, double inv_n, float eps) {
     const double m = s * inv_n;
-    const float v = fmaxf((float)(q * inv_n - m * m), 0.f);
-    return make_float2((float)m, rsqrtf(v + eps));
+    const float v = (float)(q * inv_n - m * m);
+    return make_float2((float)m, rsqrtf((v < 0.f ? 0.f : v) + eps));   // (a NaN stays one)
 }
 
 // V consecutive floats at any alignment of 4 bytes, 16 bytes at a time
