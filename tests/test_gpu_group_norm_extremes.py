@@ -52,3 +52,20 @@ def test_a_diverged_group_shows(ops, B, n, C, G, dt, bad):
     stats = torch.zeros(B, G, dtype=torch.bool, device="cuda")
     stats[0, -1] = True
     assert torch.equal(mean[~stats], wm[~stats]) and torch.equal(rstd[~stats], wr[~stats])
+
+
+def test_statistics_of_many_rows_a_thread(ops):
+    """256 images of 1024 rows, one group of 2048: a thread walks a thousand rows of ones, the second half 2^-17 larger.  Added row by
+    row, each of those small steps is below half a step of the mean in fp32, and the mean would stay where it was."""
+    B, n, C = 256, 1024, 2048
+    x = torch.ones(B, n, C, device="cuda")
+    x[:, n // 2:] += 2.0 ** -17
+    one, zero = torch.ones(C, device="cuda"), torch.zeros(C, device="cuda")
+    y, mean, _, _ = forward(ops, x.view(B * n, C), one, zero, B, n, C, 1)
+    assert float((mean.double() - (1 + 2.0 ** -18)).abs().max()) <= 4 * U
+    r = (2.0 ** -36 + EPS) ** -0.5
+    want = 2.0 ** -18 * r
+    # the file's 16 u (|m a| + |(x - m) a|) with a = r
+    tol = 16 * U * (r + want) + U * want
+    y = y.view(B, n, C)
+    assert float((y[:, :n // 2] + want).abs().max()) <= tol and float((y[:, n // 2:] - want).abs().max()) <= tol

@@ -19,6 +19,7 @@ namespace {
 constexpr int GN_T = 512;          // threads of the streaming kernels
 constexpr int GN_R = 8;            // rows a thread of the resident form holds
 constexpr int GN_RS = 4;           // rows a thread of the streamed form loads ahead of using them
+constexpr int GN_RUN = 128;        // rows that a thread of the streamed form adds up in fp32 before the sums move on to fp64
 constexpr int GN_MAX_C = 2048;     // channels of a group, and so of a slab, are bounded by the per-slab sums in LDS
 constexpr int GN_MAX_CHUNKS = 128; // row chunks of an image (each output block sums all partials of its slab)
 
@@ -336,29 +337,34 @@ __global__ void __launch_bounds__(GN_T) gn_stats_kernel(GnArgs p) {
     for (int v0 = 0; v0 < l.tw; v0 += GN_T) {
         const bool wide = l.tw > GN_T;
         const int cv = wide ? v0 + tid : l.cv;
-        Stat<V> st;
-        st.clear();
-        if (wide ? cv < l.tw : l.rl < l.RL) {
-            const TX* src = X + (size_t)cv * V;
-            row_batches<GN_RS>(r0 + (wide ? 0 : l.rl), r1, l.RL, [&](int r, int k) {
-                Pack<TX, V> buf[GN_RS];
-                load_rows<GN_RS>(buf, src, p.ldx, r, l.RL, k);
-                st.template batch<GN_RS>(buf, k);
-            });
-        }
-        if (wide) {   // a single group: the thread's own sums
+        const TX* src = X + (size_t)cv * V;
+        int g0 = r0;
+        do {   // runs of GN_RUN rows a thread (one but for many large images; none where a chunk is empty)
+            const int g1 = min(r1, g0 + l.RL * GN_RUN);
+            Stat<V> st;
+            st.clear();
+            if (wide ? cv < l.tw : l.rl < l.RL)
+                row_batches<GN_RS>(g0 + (wide ? 0 : l.rl), g1, l.RL, [&](int r, int k) {
+                    Pack<TX, V> buf[GN_RS];
+                    load_rows<GN_RS>(buf, src, p.ldx, r, l.RL, k);
+                    st.template batch<GN_RS>(buf, k);
+                });
+            if (wide) {   // a single group: the thread's own sums
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const double k = st.cnt, m = st.mean[j];
-                wide_s += k * m;
-                wide_q += (double)st.m2[j] + k * m * m;
+                for (int j = 0; j < V; ++j) {
+                    const double k = st.cnt, m = st.mean[j];
+                    wide_s += k * m;
+                    wide_q += (double)st.m2[j] + k * m * m;
+                }
+                continue;
             }
-            continue;
-        }
-        const int fold = fold_of<V>(p.cg);
-        put_stats(st, fold, tid, sm, sq);
-        slab_group_sums<GN_T, V>(p, l, fold, r1 - r0, sm, sq, scratch, tid,
-                                 [&](int g, double s, double q) { out[(size_t)g * p.chunks] = make_double2(s, q); });
+            const int fold = fold_of<V>(p.cg);
+            put_stats(st, fold, tid, sm, sq);
+            slab_group_sums<GN_T, V>(p, l, fold, g1 - g0, sm, sq, scratch, tid, [&](int g, double s, double q) {
+                double2& o = out[(size_t)g * p.chunks];   // the same thread's every time
+                o = g0 == r0 ? make_double2(s, q) : make_double2(o.x + s, o.y + q);
+            });
+        } while ((g0 += l.RL * GN_RUN) < r1);
     }
     if (l.tw > GN_T) {
         double2* all = scratch + GN_T / 64;   // [GN_T], in the place of sm and sq
