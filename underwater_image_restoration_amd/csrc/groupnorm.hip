@@ -475,7 +475,7 @@ __device__ __forceinline__ void bwd_stats(const GnArgs& p, Coef<V>& co, int b, i
     each_group<V>(c0, p.cg, [&](int j, int g) { co.stats(j, m[g], r[g]); });
 }
 
-// adds a batch of rows: s1 += sum dz, s2 += sum dz d.  A short chain per batch keeps the fp32 sums close to pairwise.
+// adds a batch of rows: s1 += sum dz, s2 += sum dz d, each summed within the batch first
 template <int R, typename T, int V>
 __device__ __forceinline__ void bwd_batch(const Pack<T, V>* bx, const Pack<T, V>* bd, const Coef<V>& co, int k, bool silu, float* s1,
                                           float* s2) {
@@ -523,7 +523,8 @@ constexpr int GN_RB = 2;   // rows a thread has in flight, x and dy each: coeffi
 template <typename T, int V>
 __global__ void __launch_bounds__(GN_T, 4) gn_bwd_sums_kernel(GnArgs p) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    float2* red = reinterpret_cast<float2*>(smem);   // [GN_T][V]
+    float2* red = reinterpret_cast<float2*>(smem);             // [GN_T][V]
+    double2* run = reinterpret_cast<double2*>(red + GN_T * V); // [slab]
     const int tid = threadIdx.x, chunk = blockIdx.x, b = blockIdx.z;
     const Place l = Place::of<V>(p, blockIdx.y, b, tid, GN_T);
     const int r0 = chunk * p.rows, r1 = min(p.n, r0 + p.rows);
@@ -534,48 +535,66 @@ __global__ void __launch_bounds__(GN_T, 4) gn_bwd_sums_kernel(GnArgs p) {
     for (int v0 = 0; v0 < l.tw; v0 += GN_T) {
         const bool wide = l.tw > GN_T;
         const int cv = wide ? v0 + tid : l.cv;
-        float s1[V], s2[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) s1[j] = s2[j] = 0.f;
-        if (wide ? cv < l.tw : l.rl < l.RL) {
-            Coef<V> co;
-            bwd_stats<V, T>(p, co, b, l.ch0 + cv * V);
-            row_batches<GN_RB>(r0 + (wide ? 0 : l.rl), r1, l.RL, [&](int r, int k) {
-                Pack<T, V> bx[GN_RB], bd[GN_RB];
-                load_rows<GN_RB>(bx, X + cv * V, p.ldx, r, l.RL, k);
-                load_rows<GN_RB>(bd, DY + cv * V, p.ldy, r, l.RL, k);
-                bwd_batch<GN_RB>(bx, bd, co, k, silu, s1, s2);
-            });
-#pragma unroll
-            for (int j = 0; j < V; ++j) s2[j] *= co.r[j];
-        }
-        if (wide) {
-            if (cv < l.tw)
-#pragma unroll
-                for (int j = 0; j < V; ++j) out[cv * V + j] = make_float2(s1[j], s2[j]);
-            continue;
-        }
-#pragma unroll
-        for (int j = 0; j < V; ++j) red[tid * V + j] = make_float2(s1[j], s2[j]);
-        __syncthreads();
-        // a team of T / width threads per channel (a power of two within a wave) over the row lanes
-        int team = 1;
-        while (team < 64 && team * 2 * l.sc <= GN_T) team *= 2;
-        for (int c0 = 0; c0 < l.sc; c0 += GN_T / team) {
-            const int c = c0 + tid / team;
-            double a = 0., q = 0.;
-            if (c < l.sc)
-                for (int i = tid & (team - 1); i < l.RL; i += team) {
-                    const float2 v = red[i * l.sc + c];
-                    a += v.x;
-                    q += v.y;
+        const bool mine = wide ? cv < l.tw : l.rl < l.RL;
+        Coef<V> co;
+        if (mine) bwd_stats<V, T>(p, co, b, l.ch0 + cv * V);
+        int g0 = r0;
+        bool more;
+        do {   // runs of GN_RUN rows a thread (one but for many large images; none where a chunk is empty)
+            const int g1 = min(r1, g0 + l.RL * GN_RUN);
+            more = g0 + l.RL * GN_RUN < r1;
+            // a channel's sums: to memory after the last run, into `run` (by the same thread every time) before
+            auto put = [&](int c, double a, double q) {
+                if (g0 != r0) {
+                    a += run[c].x;
+                    q += run[c].y;
                 }
-            for (int o = team >> 1; o; o >>= 1) {
-                a += shfl_xor_d(a, o);
-                q += shfl_xor_d(q, o);
+                if (more) run[c] = make_double2(a, q);
+                else out[c] = make_float2((float)a, (float)q);
+            };
+            float s1[V], s2[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) s1[j] = s2[j] = 0.f;
+            if (mine) {
+                row_batches<GN_RB>(g0 + (wide ? 0 : l.rl), g1, l.RL, [&](int r, int k) {
+                    Pack<T, V> bx[GN_RB], bd[GN_RB];
+                    load_rows<GN_RB>(bx, X + cv * V, p.ldx, r, l.RL, k);
+                    load_rows<GN_RB>(bd, DY + cv * V, p.ldy, r, l.RL, k);
+                    bwd_batch<GN_RB>(bx, bd, co, k, silu, s1, s2);
+                });
+#pragma unroll
+                for (int j = 0; j < V; ++j) s2[j] *= co.r[j];
             }
-            if (c < l.sc && (tid & (team - 1)) == 0) out[c] = make_float2((float)a, (float)q);
-        }
+            if (wide) {
+                if (mine)
+#pragma unroll
+                    for (int j = 0; j < V; ++j) put(cv * V + j, s1[j], s2[j]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j) red[tid * V + j] = make_float2(s1[j], s2[j]);
+                __syncthreads();
+                // a team of T / width threads per channel (a power of two within a wave) over the row lanes
+                int team = 1;
+                while (team < 64 && team * 2 * l.sc <= GN_T) team *= 2;
+                for (int c0 = 0; c0 < l.sc; c0 += GN_T / team) {
+                    const int c = c0 + tid / team;
+                    double a = 0., q = 0.;
+                    if (c < l.sc)
+                        for (int i = tid & (team - 1); i < l.RL; i += team) {
+                            const float2 v = red[i * l.sc + c];
+                            a += v.x;
+                            q += v.y;
+                        }
+                    for (int o = team >> 1; o; o >>= 1) {
+                        a += shfl_xor_d(a, o);
+                        q += shfl_xor_d(q, o);
+                    }
+                    if (c < l.sc && (tid & (team - 1)) == 0) put(c, a, q);
+                }
+                if (more) __syncthreads();
+            }
+            g0 += l.RL * GN_RUN;
+        } while (more);
     }
 }
 
@@ -907,7 +926,8 @@ template <typename T, int V> void launch_bwd(GnArgs p, hipStream_t st) {
     }
     stream_shape(p, V, sizeof(T));
     const int slabs = ceil_div(p.C, p.slab);
-    hipLaunchKernelGGL((gn_bwd_sums_kernel<T, V>), dim3(p.chunks, slabs, p.B), dim3(GN_T), (size_t)GN_T * V * 8, st, p);
+    hipLaunchKernelGGL((gn_bwd_sums_kernel<T, V>), dim3(p.chunks, slabs, p.B), dim3(GN_T),
+                       (size_t)GN_T * V * 8 + (size_t)p.slab * 16, st, p);
     p.sums = p.cpart;
     p.sum_chunks = p.chunks;
     if (p.slab * p.chunks > 8192) {   // 64 KB of partials a block: sum them once instead
