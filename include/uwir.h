@@ -291,11 +291,13 @@ int uwir_group_norm_act_backward(const void* dy, size_t ldy, const void* x, size
  * scale q k each within +-1e38, nk max |v| below 8e34 (a row that meets a NaN or an infinity is unspecified, other rows
  * are not touched by a bad query).  k and v of an invisible key are never used,
  * whatever they hold; their gradients are written as zeros.  backward: dq, dk, dv (written, not added to) from out, lse of
- * the forward call and dout (sum_d dout out is formed from p and dout v^T instead where bf16 keys are at most 256); the gradients of shared key heads are summed over their query heads in a fixed order.
+ * the forward call and dout (sum_d dout out is formed from p and dout v^T instead where bf16 keys are at most 256); the
+ * gradients of shared key heads are summed over their query heads in a fixed order.
  * All tensors of a call share a dtype (fp32: exact-fp32 MFMA; bf16: bf16 MFMA operands with probabilities and score
  * gradients rounded to bf16, fp32 accumulation and statistics).  hd % 8 == 0, hd <= 128; rows and strides 16-byte aligned;
- * 1e-20 <= scale <= 1e20; row strides below 32 MB; nq, nk >= 0; B * kv_heads <= 65535.  Outputs, lse and the workspace must not share memory with another operand (column ranges of one
- * wider matrix that do not meet are fine).
+ * 1e-20 <= scale <= 1e20; row strides below 32 MB; nq, nk >= 0; B * kv_heads <= 65535.  Outputs, lse and the workspace
+ * must not share memory with another operand, key_lens and key_mask included (q, k, v, out, dout and gradients may be
+ * column ranges of one wider matrix that do not meet).
  * workspace: >= the matching *_workspace_bytes (may be 0), 16-byte aligned; calls that may run at the same
  * time need one each (captured graphs included).  Results do not depend on scheduling. */
 size_t uwir_cross_attn_workspace_bytes(int B, int nq, int nk, int heads, int kv_heads, int hd, int dtype);

@@ -268,4 +268,24 @@ inline int xattn_check_apart(const char* what, const char* name, const void* p, 
     return UWIR_OK;
 }
 
+// key_lens and key_mask are read while the call writes: neither may meet an output, nor the memory `extra` written beside them.
+struct XRange {
+    const void* p;
+    size_t n;
+    const char* name;
+};
+inline int xattn_check_keys(const char* what, const int* lens, const unsigned char* mask, size_t ldm, int B, int nk, int dtype, int hd,
+                            const XMat* out, int n_out, const XRange* extra, int n_extra) {
+    const XRange in[] = {{lens, (size_t)B * sizeof(int), "key_lens"}, {mask, nk ? (size_t)(B - 1) * ldm + nk : 0, "key_mask"}};
+    for (const XRange& r : in) {
+        if (!r.p || !r.n) continue;
+        if (int rc = xattn_check_apart(what, r.name, r.p, r.n, dtype, hd, out, n_out)) return rc;
+        for (int i = 0; i < n_extra; ++i) {
+            const uintptr_t x = (uintptr_t)r.p, y = (uintptr_t)extra[i].p;
+            UWIR_CHECK(!extra[i].p || !extra[i].n || x + r.n <= y || y + extra[i].n <= x, "%s: %s overlaps %s", what, extra[i].name, r.name);
+        }
+    }
+    return UWIR_OK;
+}
+
 }  // namespace

@@ -533,6 +533,8 @@ extern "C" int uwir_cross_attn(const void* q, size_t ldq, const void* k, size_t 
     }
     const uintptr_t w = (uintptr_t)workspace, l = (uintptr_t)lse;
     UWIR_CHECK(!need || !lse || w + need <= l || l + nl <= w, "cross_attn: the workspace overlaps lse");
+    const XRange beside[] = {{workspace, need, "the workspace"}, {lse, nl, "lse"}};
+    if (int rc = xattn_check_keys("cross_attn", key_lens, key_mask, ld_mask, B, nk, dtype, hd, res, 1, beside, 2)) return rc;
     const Plan pl = plan_fwd(B, nq, nk, heads, kv_heads, hd, dtype);
     XArgs p = {};
     p.q = q; p.k = k; p.v = v; p.o = out; p.lse = lse; p.lens = key_lens; p.mask = key_mask;

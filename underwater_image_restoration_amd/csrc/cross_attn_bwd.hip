@@ -855,6 +855,8 @@ extern "C" int uwir_cross_attn_backward(const void* q, size_t ldq, const void* k
     if (int rc = xattn_check_apart("cross_attn_backward", "lse", lse, (size_t)B * heads * nq * sizeof(float), dtype, hd, res, 3)) return rc;
     const uintptr_t w = (uintptr_t)workspace, ls = (uintptr_t)lse;
     UWIR_CHECK(!nq || w + need <= ls || ls + (size_t)B * heads * nq * sizeof(float) <= w, "cross_attn_backward: the workspace overlaps lse");
+    const XRange beside[] = {{workspace, need, "the workspace"}};
+    if (int rc = xattn_check_keys("cross_attn_backward", key_lens, key_mask, ld_mask, B, nk, dtype, hd, res, 3, beside, 1)) return rc;
     const size_t apart = (ldq > ld_dout ? ldq : ld_dout) * (dtype == UWIR_BF16 ? 2 : 4);
     const Plan pl = plan_bwd(B, nq, nk, heads, kv_heads, hd, dtype, key_lens != nullptr, apart >= (1u << 24));
     const Layout lo = layout(pl, B, nq, nk, heads, kv_heads, hd);
