@@ -1,7 +1,9 @@
 """CPU: calls of group_norm_act / cross_attn beyond the sizes that the kernels' indexes hold, or with written memory on an operand that is
 read beside the rows.  Refused before any HIP call."""
 import pytest
+import torch
 
+from underwater_image_restoration_amd import ops
 from tests.test_norm_attn_refusals import GN_APART, GNB_APART, P, SPLIT, ca, cab, gn, gnb, refused
 
 
@@ -27,3 +29,11 @@ def test_cross_attn_refuses_lengths_and_masks_in_written_memory(kw, words):
     (dict(lens=P << 8), ("workspace", "key_lens")), (dict(mask=P << 8, ldm=64), ("workspace", "key_mask"))])
 def test_cross_attn_backward_refuses_lengths_and_masks_in_written_memory(kw, words):
     refused(cab(**dict(dict(lse=P << 10), **kw)), "cross_attn_backward", "overlaps", *words)
+
+
+def test_host_operands_are_named_in_the_error():
+    q, k = torch.zeros(10, 64), torch.zeros(20, 64)
+    with pytest.raises(ValueError, match="operand on cpu: every operand of an op is a tensor on the current HIP device"):
+        ops.cross_attn(q, k, k, 2, 5, 10, 2, 2, 32, 0.5, torch.zeros(10, 64), None)
+    with pytest.raises(ValueError, match="operand on meta: every operand"):
+        ops._stream(torch.device("meta"))

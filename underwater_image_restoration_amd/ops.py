@@ -20,11 +20,13 @@ def _stream(t) -> int:
     another GPU is an error here (it used to enqueue on the wrong GPU's stream silently).  The module-level entry
     points (student / UNet / DA-CLIP / sampler forwards) make their input's device current themselves."""
     dev = t.device if isinstance(t, torch.Tensor) else t
-    cur = torch._C._cuda_getDevice() if dev.type == "cuda" else None   # what torch.cuda.current_stream() asks, without its
-    if cur is None or (dev.index is not None and dev.index != cur):     # Stream object: 3 us a launch
-        raise ValueError(f"operand on {dev} but the current HIP device is {'not asked' if cur is None else f'cuda:{cur}'}: run "
-                         f"under torch.cuda.device(...) (the model-level forwards do)")
-    return torch._C._cuda_getCurrentRawStream(cur)
+    if dev.type != "cuda":
+        raise ValueError(f"operand on {dev}: every operand of an op is a tensor on the current HIP device")
+    cur = torch.cuda.current_device()
+    if dev.index is not None and dev.index != cur:
+        raise ValueError(f"operand on {dev} but the current HIP device is cuda:{cur}: run under torch.cuda.device(...) "
+                         f"(the model-level forwards do)")
+    return torch._C._cuda_getCurrentRawStream(cur)   # torch.cuda.current_stream().cuda_stream without its Stream object: 3 us a launch
 
 
 def on_operand_device(fn):
