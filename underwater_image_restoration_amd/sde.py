@@ -251,9 +251,10 @@ class IRSDE:
         # the context tensors and the model's weights are not modified while the loop runs (the schedule notices an
         # in-place edit of a context through tensor._version and then recomputes per step like the reference)
         sched = getattr(self.model, "conditioning_schedule", None)
-        ok = sched is not None and x.is_cuda and set(kwargs) <= {"text_context", "image_context"}
-        ctx = (sched([t * self.sample_scale for t in range(1, T + 1)], x.shape[0], device=x.device, **kwargs) if ok
-               else contextlib.nullcontext())
+        # (context_lens only says which states the attention reads: nothing of the schedule depends on it)
+        ok = sched is not None and x.is_cuda and set(kwargs) <= {"text_context", "image_context", "context_lens"}
+        ctx = (sched([t * self.sample_scale for t in range(1, T + 1)], x.shape[0], device=x.device,
+                     **{k: v for k, v in kwargs.items() if k != "context_lens"}) if ok else contextlib.nullcontext())
         with ctx:
             for i, t in enumerate(reversed(range(1, T + 1))):
                 pred = self.noise_fn(x, t, self.sample_scale, **kwargs)
