@@ -643,7 +643,7 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 // Denominators when the V^T tile has no spare row for a ones row (LSV): 0 = a ones-operand 32x32x16 MFMA per 16 keys
 // (every one of its 32 output rows is the same sum: 64 MFMA cycles per 32 x 32 block); 1 = fp32 adds of the
-// exponentials on the VALU (8 per block, on the pipe that bounds this kernel); 2 = a 16x16x32 MFMA whose A operand is
+// exponentials on the VALU (16 per block, on the pipe that bounds this kernel); 2 = a 16x16x32 MFMA whose A operand is
 // a 0/1 selector: fed the 32x32x16 B fragment as it is, lane group G of its k dimension holds queries 16 (G & 1) + n,
 // key half G >> 1, so row 0 = groups {0, 2} and row 1 = groups {1, 3} give the sums of queries n and n + 16: half the
 // MFMA cycles of (0) and no VALU work.
@@ -967,8 +967,8 @@ static int launch_attn_packed(const AttnP& p, int B, void* workspace, hipStream_
     const long long nb = (long long)nqb * p.heads * B;
     if (nb > 0x7fffffffLL) return uwir_set_error(UWIR_EINVAL, "flash_attn: grid too large");
     probe_mark(0, stream);
-    // measured (tools/bench_attn.py lsv): hd16 2V 2.18 / 2.02 / 1.83 ms for forms 0 / 1 / 2, hd32 1V 0.53 / 0.51 / 0.47,
-    // hd32 2V 0.258 / 0.223 / 0.234
+    // measured (tools/bench_attn.py lsv): hd16 2V 2.15 / 1.94 / 1.85 ms for forms 0 / 1 / 2, hd32 1V 0.59 / 0.497 / 0.470,
+    // hd32 2V 0.266 / 0.226 / 0.237
     const int lsv = P::SUMROW ? 0 : (!attn_lsv_forced() ? ((HD == 32 && NV == 2) ? 1 : 2) : (g_attn_lsv & 3));
     const unsigned cap = attn_cap_lds();
     const dim3 grid((unsigned)nb);

@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(256) dwconv_ms_kernel(const TIN* __restrict__ 
 // ------------------------------------------------------------------------------------------
 // Second form (C % 32 == 0): the kernel above reads 83 weight quads + 70 input quads from LDS per thread and is bound
 // by LDS bandwidth, not by its FMAs.  Here a WAVE owns one channel quad, so the 83 x 4 weights of the quad are
-// wave-uniform and arrive through scalar loads (SGPR operands of the packed FMAs): LDS carries the input rows only.
+// wave-uniform and arrive through scalar loads (SGPR operands of the FMAs): LDS carries the input rows only.
 // Block = 8 waves = 32 channels over a 16 x 16 pixel tile; lane = (row y, 4-pixel group xg); the 22 x 22 halo tile sits
 // in LDS as one fp32 plane per quad with an odd row pitch (23 quads), which makes the 16 row-lanes of a 16-byte LDS
 // read hit 16 distinct bank groups.  A lane's results are 8-byte pieces scattered over 12 (pixel, scale) rows, so bf16
@@ -143,7 +143,8 @@ __global__ void __launch_bounds__(256) dwconv_ms_kernel(const TIN* __restrict__ 
 #define D2_OPS 104                  // bf16 elements per staged output pixel: 3 x 32 + 8 pad (208 B: 16-byte aligned, and
                                     // 16 row-lanes x 208 B land on 16 distinct bank groups)
 
-// Measured on MI355X (tools/exp/dw_phases.hip, level-0 shape 16 x 128 x 128 x 576): loads only 0.12 ms, FMAs only
+// Measured on MI355X (tools/exp/dw_phases.hip, level-0 shape 16 x 128 x 128 x 576, then with packed FMAs at twice the
+// rate of the single ones it is built with now): loads only 0.12 ms, FMAs only
 // 0.24 ms, stores only 0.16 ms above the empty kernel -- and the one-tile-per-block form took their SUM (0.62 ms): the
 // resident blocks run in lock step chip-wide, so the memory phases (HBM-bound while they last) and the FMA phase never
 // overlap.  Hence a block walks `nt` consecutive tiles, software-pipelined: the next tile's halo is fetched into
@@ -370,9 +371,11 @@ static int launch_dw(const void* x, int ldx, int B, int H, int W, int C, const f
         (long long)ceil_div(W, D2_T) * ceil_div(H, D2_T) <= 65535 &&
         (size_t)H * W * ldx * sizeof(TIN) < 0x7fffffffULL && (size_t)H * W * ldo * sizeof(TOUT) < 0x7fffffffULL) {
         const int tx = ceil_div(W, D2_T), ty = ceil_div(H, D2_T), tiles = tx * ty;
-        // tiles per block: enough blocks left for >= 8 rounds of the chip's 512 resident blocks
+        // tiles per block: two where two rounds of the chip's 512 resident blocks are left.  More do not pay since the FMAs are issued
+        // one by one: 16 x 128 x 128 x 576 0.617 ms with two tiles a block, 0.638 with four, 0.663 with one; 16 x 64 x 64 x 1152
+        // 0.325, 0.334 and 0.350; 16 x 32 x 32 x 2304 0.166, 0.180 and 0.180
         const long long nblk = (long long)(C / 32) * tiles * B;
-        const int nt = g_dw_nt ? g_dw_nt : (nblk >= 16384 ? 4 : (nblk >= 8192 ? 3 : (nblk >= 2048 ? 2 : 1)));
+        const int nt = g_dw_nt ? g_dw_nt : (nblk >= 2048 ? 2 : 1);
         const dim3 grid(C / 32, ceil_div(tiles, nt), B);
         if (in_scale)
             hipLaunchKernelGGL((dwconv_ms32_kernel<TIN, TOUT, true>), grid, dim3(512), 0, stream, (const TIN*)x, ldx, H, W, C,
