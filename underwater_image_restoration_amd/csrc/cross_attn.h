@@ -179,6 +179,21 @@ inline Divisor make_divisor(unsigned d) {
     return v;
 }
 
+template <typename T, int HD> struct Tile {
+    typedef Mma<T> M;
+    static constexpr int VEC = M::VEC, STR = HD + M::PAD, CPR = HD / VEC;   // 16-byte chunks per row
+};
+
+// the row of q / out that packed row r of key head kv stands for; Args: B, nq, G and by_g of either direction
+struct RowRef {
+    size_t row;
+    int head;
+};
+template <typename Args> __device__ __forceinline__ RowRef row_ref(const Args& p, int b, int kv, int r) {
+    const int qi = (int)p.by_g.quot((unsigned)r);
+    return {(size_t)b * p.nq + qi, kv * p.G + (r - qi * p.G)};
+}
+
 // Which (head, image, part, tile) a block works on.  Heads next to each other: the blocks that run together read whole rows.
 // Then, an XCD taking a contiguous range of the order: with all images of one length the images far apart, so that an XCD holds
 // few images' keys in its L2; with lengths of their own next to each other, so that every XCD gets its share of the long ones.
@@ -207,8 +222,11 @@ __device__ __forceinline__ Item block_item(unsigned vid, int KV, int B, int part
 
 }  // namespace xattn
 
-// ---- host side: argument checks shared by both directions
+// ---- host side: sizes and argument checks shared by both directions
 namespace {
+
+inline int hd_class(int hd) { return hd <= 32 ? 32 : hd <= 64 ? 64 : 128; }
+inline size_t al256(size_t v) { return (v + 255) & ~(size_t)255; }
 
 struct XMat {
     const void* p;

@@ -33,21 +33,6 @@ struct XArgs {
     float m0;           // the running reference before any key is seen: low, and m0 * c finite
 };
 
-template <typename T, int HD> struct Tile {
-    typedef Mma<T> M;
-    static constexpr int VEC = M::VEC, STR = HD + M::PAD, CPR = HD / VEC;   // 16-byte chunks per row
-};
-
-// the row of q / out that packed row r of key head kv stands for
-struct RowRef {
-    size_t row;
-    int head;
-};
-__device__ __forceinline__ RowRef row_ref(const XArgs& p, int b, int kv, int r) {
-    const int qi = (int)p.by_g.quot((unsigned)r);
-    return {(size_t)b * p.nq + qi, kv * p.G + (r - qi * p.G)};
-}
-
 // One 32-row group of a wave: running maximum m (raw scores), this lane's part of the sum, O^T.
 template <typename T, int HD> struct Group {
     typedef Mma<T> M;
@@ -458,8 +443,6 @@ struct Plan {
     int qtiles, splits;
 };
 
-int hd_class(int hd) { return hd <= 32 ? 32 : hd <= 64 ? 64 : 128; }
-
 Plan plan_fwd(int B, int nq, int nk, int H, int KV, int hd, int dtype) {
     Plan pl = {};
     const long long R = (long long)nq * (H / KV), bk = (long long)B * KV;
@@ -500,8 +483,6 @@ template <typename T, int HD> void launch(const XArgs& p, const Plan& pl, hipStr
         hipLaunchKernelGGL((xattn_join_kernel<T>), dim3((unsigned)ceil_div_sz(n, 256)), dim3(256), 0, st, p);
     }
 }
-
-size_t al256(size_t v) { return (v + 255) & ~(size_t)255; }
 
 }  // namespace
 

@@ -30,20 +30,6 @@ struct BArgs {
     float c, scale;
 };
 
-template <typename T, int HD> struct Tile {
-    typedef Mma<T> M;
-    static constexpr int VEC = M::VEC, STR = HD + M::PAD, CPR = HD / VEC;
-};
-
-struct RowRef {
-    size_t row;
-    int head;
-};
-__device__ __forceinline__ RowRef row_ref(const BArgs& p, int b, int kv, int r) {
-    const int qi = (int)p.by_g.quot((unsigned)r);
-    return {(size_t)b * p.nq + qi, kv * p.G + (r - qi * p.G)};
-}
-
 __device__ __forceinline__ int image_len(const BArgs& p, int b) {
     return p.lens ? max(0, min(p.nk, p.lens[b])) : p.nk;
 }
@@ -719,8 +705,6 @@ struct Plan {
     int qsplits, qtiles, kw, ksplits, ktiles;
 };
 
-int hd_class(int hd) { return hd <= 32 ? 32 : hd <= 64 ? 64 : 128; }
-
 // parts of an axis of `tiles` steps so that `blocks` blocks grow to about two per CU, each with two steps at least
 int parts(long long blocks, long long tiles) {
     long long s = blocks >= 384 ? 1 : (512 + blocks - 1) / (blocks > 0 ? blocks : 1);
@@ -754,8 +738,6 @@ Plan plan_bwd(int B, int nq, int nk, int H, int KV, int hd, int dtype, bool ragg
     pl.ksplits = parts(bk * pl.ktiles, (R + 63) / 64);
     return pl;
 }
-
-size_t al256(size_t v) { return (v + 255) & ~(size_t)255; }
 
 struct Layout {
     size_t ld, q, k, v, total;
