@@ -88,7 +88,7 @@ template <int V> struct Stat {
             }
             const float d = m - mean[j];
             mean[j] = fmaf(d, wa, mean[j]);
-            m2[j] += cnt ? fmaf(d * d, wb, q) : q;   // of the first batch d is the mean itself: its square may leave the range
+            m2[j] += fmaf(d, d * wb, q);   // of the first batch d is the mean itself, whose square may leave the range, and wb 0
         }
         cnt += k;
     }
