@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from tests.test_gpu_cross_attn import BF, F32, U, check, inputs, ops  # noqa: F401
+from tests.test_gpu_cross_attn import BF, F32, U, check, close, inputs, ops, reference  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -92,3 +92,22 @@ def test_large_values_under_rising_scores(ops, dims, dt):
     t["q"], t["k"] = q.reshape(B * nq, -1).to(dt), k.reshape(B * nk, -1).to(dt)
     t["v"] = (t["v"].float() * 1e22).to(dt)
     check(ops, t, dims, grads=nq < 100)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("dt", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("dims", [(2, 5, 300, 4, 2, 64), (2, 300, 77, 4, 2, 32), (2, 300, 400, 2, 2, 96), (8, 2053, 300, 8, 8, 24)],
+                         ids=lambda d: "x".join(map(str, d)))
+def test_a_bad_query_stays_in_its_row(ops, dims, dt, bad):
+    """A query row of NaN or infinities (and a gradient row) leaves the answers and dq of all other rows right."""
+    B, nq, nk, H, KV, hd = dims
+    t = inputs(*dims, "mask", dt, seed=13)
+    rows = torch.tensor([0, nq + nq // 2, B * nq - 1], device="cuda")
+    ok = torch.ones(B * nq, dtype=torch.bool, device="cuda")
+    ok[rows] = False
+    hit = dict(t, q=t["q"].clone(), do=t["do"].clone())
+    hit["q"][rows] = bad
+    hit["do"][rows] = bad
+    r, w = reference(t, *dims), call(ops, hit, dims, hd ** -0.5)
+    close("out", w["out"][ok], r["o"][ok], r["to"][ok], r["h"])
+    close("dq", w["dq"][ok], r["dq"][ok], r["tdq"][ok], r["h"])

@@ -85,3 +85,32 @@ def test_gradients_of_many_rows_a_thread(ops):
     ops.group_norm_act_backward(dy, x, B, n, C, 1, one, zero, mean, rstd, dy, dg, db, ws, scale_shift=ss, dscale_shift=dss)
     for got, want in ((dss, n * d), (dg, B * n * d), (db, B * n * d)):
         assert float((got.double() - want).abs().max()) <= 66 * U * want
+
+
+# so many images that a block has all rows of one: several runs of 128 rows a thread, the last ones ragged; one group wider than a block,
+# vectors of 16 bytes and the most LDS, several groups a slab
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("B,n,C,G", [(256, 300, 2047, 1), (257, 601, 2048, 1), (256, 400, 1024, 2), (256, 70001, 24, 3), (256, 33100, 32, 8)])
+def test_runs_of_rows(ops, B, n, C, G, dt):
+    """y has one tolerance more than test_gpu_group_norm_act.py's: s = beta (1 + scale) + shift with 1 + scale rounded to fp32 is off by
+    u |beta (1 + scale)|, however small s is where the two parts cancel (half a million channels and images have some that do), and
+    |act'| <= 1.1 takes that to y."""
+    x, gamma, beta, ss, dy = make(B, n, C, True, dt, seed=n)
+    y, mean, rstd, ws = forward(ops, x, gamma, beta, B, n, C, G, act=ops.ACT_SILU, ss=ss)
+    dx, dg, db, dss = torch.empty_like(x), torch.empty(C, device="cuda"), torch.empty(C, device="cuda"), torch.empty(B, 2 * C, device="cuda")
+    ops.group_norm_act_backward(dy, x, B, n, C, G, gamma, beta, mean, rstd, dx, dg, db, ws, act=ops.ACT_SILU, scale_shift=ss,
+                                dscale_shift=dss)
+    sums = dict(dgamma=0, tdgamma=0, dbeta=0, tdbeta=0)
+    for b in range(B):
+        rows = slice(b * n, (b + 1) * n)
+        r = reference(x[rows], gamma, beta, ss[b:b + 1], 1, n, C, G, True, dy=dy[rows])
+        sums = {k: v + r[k] for k, v in sums.items()}
+        if b % 51 and b != B - 1:
+            continue
+        close(y[rows], r["y"], r["ty"] + 1.1 * U * (beta * (1 + ss[b, :C])).double().abs(), HALF[dt])
+        close(mean[b:b + 1], r["mean"], 4 * U * x[rows].double().abs().max(), U)
+        close(rstd[b:b + 1], r["rstd"], 8 * U * r["rstd"], U)
+        close(dx[rows], r["dx"], r["tdx"], HALF[dt])
+        close(dss[b:b + 1], r["dss"], r["tdss"], 4 * U)
+    close(dg, sums["dgamma"], sums["tdgamma"], 4 * U)
+    close(db, sums["dbeta"], sums["tdbeta"], 4 * U)
