@@ -154,10 +154,10 @@ __device__ __forceinline__ void key_range(const XArgs& p, int b, int split, int 
 // NW waves x 32 QG rows share key tiles of KT keys in LDS (two buffers, the next tile loading meanwhile).  Nothing in a wave's way
 // through a tile overlaps its matrix and its vector work (scores, probabilities, output); the waves of a SIMD do.  With two row
 // groups a wave reads every fragment of K and V from LDS once for both: LDS, not arithmetic, held the one-group form back.
-// Bound: 8 x 128 x 128 queries over 577 states, 8 heads of 64, 224 us = 690 TF of 4 hd flops a pair.  A 32 x 32 unit takes 537
-// cycles of a SIMD: 384 to issue its vector work (16 exp at 8, the scale, the sum, the rounding), 288 of the matrix pipe; and
-// 50 us of reading q and writing out, which the blocks of a CU, equal and started together, do at the same time.
-// 8 x 32 x 32 over 50 states, 8 heads of 32: 6.0 us, latency.  fp32: one wave a SIMD at most, exact fp32 MFMA; 2 x 32 x 32 over
+// Bound: 8 x 128 x 128 queries over 577 states, 8 heads of 64, 235 us = 660 TF of 4 hd flops a pair.  A 32 x 32 unit takes 463
+// cycles of a SIMD to issue its vector work (384: 16 exp at 8, the scale, the sum, the rounding) and its 18 matrix instructions,
+// which keep the matrix pipe for 288 (both counted); and 50 us of reading q and writing out, which the blocks of a CU, equal and started together, do at the same time.
+// 8 x 32 x 32 over 50 states, 8 heads of 32: 5.9 us, latency.  fp32: one wave a SIMD at most, exact fp32 MFMA; 2 x 32 x 32 over
 // 197, 16 heads of 32, 16 us.
 template <typename T, int HD, int NW, int QG>
 __global__ void __launch_bounds__(NW * 64, QG == 2 ? 2 : 1) xattn_tile_kernel(XArgs p) {
@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(NW * 64, QG == 2 ? 2 : 1) xattn_tile_kernel(XA
 
 // R <= 32 rows: every wave walks key tiles of 32 of its own (LDS private to the wave, no block barrier in the loop).
 // Bound by reading k and v once: 16 images, one query of 32 heads over up to 8192 states of 8 heads of 64 (142 MB at these lengths)
-// 43 us with the join (6 us) from HBM, 3.4 TB/s; with one length for all images 5.0-5.3 TB/s, a copy's rate: the rest is the long
+// 42 us with the join (6 us) from HBM, 3.4 TB/s; with one length for all images 60 us (268 MB, 4.5 TB/s): the rest is the long
 // images' parts ending last.
 template <typename T, int HD>
 __global__ void __launch_bounds__(256) xattn_row_kernel(XArgs p) {

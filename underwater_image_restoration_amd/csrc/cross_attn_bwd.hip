@@ -38,7 +38,7 @@ __device__ __forceinline__ int image_len(const BArgs& p, int b) {
 // EXACT_D: D from p and dP instead of dout . out.  out is rounded to bf16, and over few keys that moves dq and dk by 0.001 of their
 // norm (0.0004 over 1500), next to 0.0017 for their own rounding; a walk more over up to 256 keys is cheap.
 // Bound by vector issue as the forward kernel is, with two products in and one out a unit: 4 x 64 x 64 queries over up to 2048 states of
-// lengths of their own, 8 heads of 64 on 2 key heads, 100 us.
+// lengths of their own, 8 heads of 64 on 2 key heads, 104 us.
 template <typename T, int HD, int QG, bool EXACT_D>
 __global__ void __launch_bounds__(256, QG == 2 ? 2 : 1) xattn_dq_kernel(BArgs p) {
     typedef Tile<T, HD> L;
@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(256, QG == 2 ? 2 : 1) xattn_dq_kernel(BArgs p)
 
 // ---------------------------------------------------------------------------------------- dk, dv
 // Bound by vector issue too: four products a unit, P and dS rounded in between, lse and D of every row read from LDS.  The same case
-// takes 140 us (410 TF of 10 hd flops a pair together with the rows kernel; 600-630 over images of one length).
+// takes 147 us (410 TF of 10 hd flops a pair together with the rows kernel; 614 over images of one length).
 // KW waves across the keys (32 each); the 4 / KW waves of one key group take the 32-row blocks of a tile in turn
 template <typename T, int HD, int KW>
 __global__ void __launch_bounds__(256) xattn_dkv_kernel(BArgs p) {

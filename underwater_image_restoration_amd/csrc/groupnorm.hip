@@ -318,7 +318,7 @@ __device__ __forceinline__ void emit(const Pack<TX, V>* buf, const Coef<V>& co, 
 }
 
 // ---------------------------------------------------------------------------------------- forward, streamed
-// Bound by reading x once: 16 x 256 x 256 x 64 bf16 (134 MB) in 22.5 us, 6.0 TB/s, 8 x 64 x 64 x 256 (17 MB) in 6.0 us.  A chunk of
+// Bound by reading x once: 16 x 256 x 256 x 64 bf16 (134 MB) in 22.2 us, 6.0 TB/s, 8 x 64 x 64 x 256 (17 MB) in 5.8 us.  A chunk of
 // rows per block, one block per CU: 3 us of every block are its start, the reductions across threads and its end.
 // A slab wider than the block (one group over more than GN_T vectors) is walked in tiles of GN_T vectors; the groups are then
 // summed tile by tile through `ch`.
@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(GN_T) gn_stats_kernel(GnArgs p) {
 
 // y = act(a x + s) with a = rstd gamma (1 + scale), s = (beta - mean rstd gamma)(1 + scale) + shift held per thread for its V
 // channels.  Bound by bytes: x again (from the memory-side cache) and y out; the first rows are loaded before the partials are
-// summed.  16 x 256 x 256 x 64 bf16 43.8 us (268 MB, 6.1 TB/s), 8 x 64 x 64 x 256 9.8 us (34 MB; the partials' sums take 3 of them).
+// summed.  16 x 256 x 256 x 64 bf16 43.8 us (268 MB, 6.1 TB/s), 8 x 64 x 64 x 256 9.3 us (34 MB; the partials' sums take 3 of them).
 template <typename TX, typename TO, int V, bool BYPASS>
 __global__ void __launch_bounds__(GN_T, 4) gn_apply_kernel(GnArgs p) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -430,7 +430,7 @@ __global__ void __launch_bounds__(GN_T, 4) gn_apply_kernel(GnArgs p) {
 
 // ---------------------------------------------------------------------------------------- forward, resident
 // All rows of a slab in a block's registers (GN_R a thread).  Bound by latency: a launch, one load, two sums across the block, one
-// store; 1 x 8 x 8 x 512 fp32 5.2 us, of which an empty kernel takes 2.
+// store; 1 x 8 x 8 x 512 fp32 5.1 us, of which an empty kernel takes 2.
 template <typename TX, typename TO, int V, int T>
 __global__ void __launch_bounds__(T) gn_resident_kernel(GnArgs p) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -466,8 +466,8 @@ __global__ void __launch_bounds__(T) gn_resident_kernel(GnArgs p) {
 }
 
 // ---------------------------------------------------------------------------------------- backward
-// SiLU's derivative costs an exponential and a reciprocal per element (8 of about 20 issue slots): it, not memory, bounds the
-// bf16 passes.  With d = x - m the sums need dz and dz d only (xh = d r enters once per channel).
+// SiLU's derivative costs an exponential and a reciprocal per element (8 of about 20 issue slots): in the bf16 passes vector work
+// takes half to two thirds of the cycles (counted), little of it under the loads with two waves a SIMD.  With d = x - m the sums need dz and dz d only (xh = d r enters once per channel).
 template <int V, typename T>
 __device__ __forceinline__ void bwd_stats(const GnArgs& p, Coef<V>& co, int b, int c0) {
     co.load(p, b, c0);
@@ -516,7 +516,7 @@ __device__ __forceinline__ void bwd_emit(const Pack<T, V>* bx, const Pack<T, V>*
 }
 
 // S1 = sum dz, S2 = sum dz xh per channel over a chunk of rows, dz = dy act'(z).  Bound by reading x and dy and, with SiLU, by the
-// exponential and reciprocal per element: 8 x 128 x 128 x 128 bf16 15.8 us (67 MB, 4.2 TB/s), 8 x 256 x 256 x 64 fp32 38.8 us
+// exponential and reciprocal per element: 8 x 128 x 128 x 128 bf16 16.3 us (67 MB, 4.1 TB/s), 8 x 256 x 256 x 64 fp32 38.8 us
 // (268 MB, 6.9 TB/s).
 constexpr int GN_RB = 2;   // rows a thread has in flight, x and dy each: coefficients fill the registers, waves hide the latency
 
@@ -646,7 +646,7 @@ __device__ __forceinline__ void affine_grads(const GnArgs& p, int tile, double2 
     }
 }
 
-// dgamma, dbeta (summed over the images in order) and dscale, dshift from the per-image sums: C B values, latency only (1.8 us)
+// dgamma, dbeta (summed over the images in order) and dscale, dshift from the per-image sums: C B values, latency only (2 us)
 __global__ void __launch_bounds__(GN_T) gn_bwd_affine_kernel(GnArgs p) {
     __shared__ double2 red[8][64];
     affine_grads(p, blockIdx.x, red);
@@ -660,7 +660,7 @@ __device__ __forceinline__ void put_dss(const GnArgs& p, int b, int c, double s1
 }
 
 // dx = rstd (w dz - m1 - xh m2), w = gamma (1 + scale), m1 and m2 the group's means of w S1 and w S2.  Bound like the sums' pass, with
-// dx to write: 21.7 us (4.6 TB/s, both reads from the memory-side cache) and 63 us (403 MB, 6.4 TB/s) at the same two sizes.
+// dx to write: 21.8 us (4.6 TB/s, both reads from the memory-side cache) and 63 us (403 MB, 6.4 TB/s) at the same two sizes.
 // output pass; the last row of blocks (b == B) forms dgamma, dbeta instead
 template <typename T, int V, bool BYPASS>
 __global__ void __launch_bounds__(GN_T, 4) gn_bwd_apply_kernel(GnArgs p) {
@@ -748,7 +748,7 @@ __global__ void __launch_bounds__(GN_T, 4) gn_bwd_apply_kernel(GnArgs p) {
 }
 
 // All rows of a slab in a block's registers, x and dy read once; per-channel sums leave for gn_bwd_affine_kernel's launch.  Bound by
-// latency: 3 x 19 x 22 x 96 fp32 7.5 us and 1.8 us.
+// latency: 3 x 19 x 22 x 96 fp32 7.6 us and 2.0 us.
 template <typename T, int V, int TH>
 __global__ void __launch_bounds__(TH) gn_bwd_resident_kernel(GnArgs p) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
