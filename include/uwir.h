@@ -266,8 +266,8 @@ int uwir_flash_attn(const void* q, int ldq, const void* k, int ldk, const void* 
  * group NaN.  mean, rstd [B, G] fp32 (each may be NULL) are what the backward pass wants kept.  out may be x itself (same stride and
  * type).  backward: dy, x, dx share a dtype; dgamma, dbeta [C] fp32 (written, not added to), dscale_shift [B, ld_dss]
  * [dscale | dshift] or NULL; dx may be dy or x itself; no other output
- * may share memory with another operand.  Statistics and sums are fp32 per thread and fp64 beyond, in a fixed order:
- * results do not depend on scheduling.  C <= 2048, B <= 65534, n < 2^30; any C, strides and element alignment (16-byte aligned
+ * may share memory with another operand.  Statistics and sums are fp32 over at most 128 rows of a thread and fp64 beyond, in a
+ * fixed order: results do not depend on scheduling.  C <= 2048, B <= 65534, n < 2^30; any C, strides and element alignment (16-byte aligned
  * rows with C a multiple of 8 (bf16) or 4 (fp32) run at full width).  workspace (both directions):
  * >= uwir_group_norm_act_workspace_bytes, 16-byte aligned, contents never carried between calls; calls that may
  * run at the same time need one each (captured graphs included). */
@@ -295,7 +295,8 @@ int uwir_group_norm_act_backward(const void* dy, size_t ldy, const void* x, size
  * gradients of shared key heads are summed over their query heads in a fixed order.
  * All tensors of a call share a dtype (fp32: exact-fp32 MFMA; bf16: bf16 MFMA operands with probabilities and score
  * gradients rounded to bf16, fp32 accumulation and statistics).  hd % 8 == 0, hd <= 128; rows and strides 16-byte aligned;
- * 1e-20 <= scale <= 1e20; row strides below 32 MB; nq, nk >= 0; B * kv_heads <= 65535.  Outputs, lse and the workspace
+ * 1e-20 <= scale <= 1e20; row strides below 32 MB; nq, nk >= 0; B * kv_heads <= 65535; nq * heads / kv_heads and nk below
+ * 2^30, and fewer than 2^24 blocks of a launch (B * heads * nq and B * kv_heads * nk below 2^30 suffice).  Outputs, lse and the workspace
  * must not share memory with another operand, key_lens and key_mask included (q, k, v, out, dout and gradients may be
  * column ranges of one wider matrix that do not meet).
  * workspace: >= the matching *_workspace_bytes (may be 0), 16-byte aligned; calls that may run at the same
